@@ -1,0 +1,342 @@
+// AdamW over every tensor of the flat space at once, with the moments held
+// in 32 or in 8 bits, and each tensor's squared norm for the trigger.
+//
+//   m' = b1 m + (1 - b1) g            v' = b2 v + (1 - b2) g^2
+//   p' = p - lr wd p - lr (m' / (1 - b1^t)) / (sqrt(v' / (1 - b2^t)) + eps)
+//   sq[i] = sum of p'^2 over tensor i
+//
+// The flat space is cut into chunks that never cross a tensor, so a block
+// has one decay and one norm. Each block leaves its part of the norm in a
+// slot of its own, and a second kernel adds the slots in a fixed order: the
+// norms, and with them the trigger's decisions, are the same on every run.
+// The step count, the learning rate and the bias corrections live on the
+// device, where the second kernel moves them on: a captured step counts
+// right on every replay.
+//
+// 8-bit moments. 64 values share one power of two, 2^(E-127), kept in a byte:
+// the one that leaves the largest of them below 2 once it is rounded up. Each
+// value is a byte on top of it: m has a sign, 4 bits of exponent and 3 behind
+// the leading one (2^-17 to 1.875), v has no sign and 5 bits of exponent
+// (2^-33 to 1.875). Values are rounded up with the probability of what lies
+// below the grid, from 16 hashed bits of (seed, step, place): with b2 = 0.999
+// a step moves v by a thousandth of itself, which rounding to the nearest of
+// 8 steps an octave would always take back. A v above zero stays above zero,
+// since m / sqrt(v) would blow up. A block with a value that is not finite
+// has E = 255 and stands for NaN throughout. E is at least 18 (m) and 34 (v):
+// every value is then a normal number in bfloat16, which holds it exactly.
+
+#include "common.h"
+
+#include <c10/core/DeviceGuard.h>
+
+namespace eg {
+namespace adamw {
+
+constexpr int BLOCK = 256;
+constexpr int QB = 64;          // values that share an exponent
+constexpr unsigned INF_BITS = 0x7f800000u;
+
+// coef: [lr, 1 / (1 - b1^t), 1 / sqrt(1 - b2^t)] of the step to come
+struct Hyper {
+  float b1, c1, b2, c2, eps;    // c = 1 - b
+  unsigned seed;
+};
+
+// m' and v' are rounded after each operation, as elementwise tensor
+// operations round them, so that a code never hangs on the compiler's choice
+// of a fused multiply-add.
+__device__ __forceinline__ float ema(float s, float b, float x, float c) {
+#pragma clang fp contract(off)
+  float a = s * b;
+  float d = x * c;
+  return a + d;
+}
+
+__device__ __forceinline__ float square(float x) {
+#pragma clang fp contract(off)
+  return x * x;
+}
+
+__device__ __forceinline__ float stepped(float p, float m, float v, float lr,
+                                         float k1, float k2, float eps,
+                                         float wd) {
+  float denom = sqrtf(v) * k2 + eps;
+  return fmaf(-lr * wd, p, p) - lr * k1 * (m / denom);
+}
+
+// ---- the 8-bit grid -------------------------------------------------------
+
+template <int EXP_BITS>
+__device__ __forceinline__ int shared_exponent(unsigned top) {
+  if (top >= INF_BITS) return 255;
+  int e = (int)((top + 0xfffffu) >> 23);
+  return min(max(e, 2 + (1 << EXP_BITS)), 254);
+}
+
+template <int EXP_BITS>
+__device__ __forceinline__ unsigned encode(float x, int e, unsigned random) {
+  constexpr int BIAS = (1 << EXP_BITS) - 1;     // of the byte's own exponent
+  float y = ldexpf(fabsf(x), 127 - e);
+  unsigned normal = ((__float_as_uint(y) + (random << 4)) >> 20) -
+                    (unsigned)((127 - BIAS) << 3);
+  // below the smallest normal: a multiple of 2^(-2 - BIAS), 16 bits further
+  unsigned low = ((unsigned)ldexpf(y, BIAS + 18) + random) >> 16;
+  unsigned q = y < ldexpf(1.f, 1 - BIAS) ? low : normal;
+  return min(q, (unsigned)((8 << EXP_BITS) - 1));
+}
+
+template <int EXP_BITS>
+__device__ __forceinline__ float decode(unsigned q, int e) {
+  constexpr int BIAS = (1 << EXP_BITS) - 1;
+  if (e == 255) return __uint_as_float(0x7fc00000u);
+  return ldexpf(__uint_as_float(q << 20), e - BIAS);
+}
+
+__device__ __forceinline__ float decode_m(unsigned byte, int e) {
+  float y = decode<4>(byte & 127u, e);
+  return byte & 128u ? -y : y;
+}
+
+__device__ __forceinline__ float decode_v(unsigned byte, int e) {
+  return decode<5>(byte, e);
+}
+
+__device__ __forceinline__ unsigned max16(unsigned v) {
+#pragma unroll
+  for (int d = 1; d < 16; d <<= 1)
+    v = max(v, (unsigned)__shfl_xor((int)v, d, 16));
+  return v;
+}
+
+// ---- the step -------------------------------------------------------------
+
+// chunks: [start, length, tensor] each; a chunk starts at a multiple of QB
+// and is taken to the next one beyond its length: the gap behind a tensor
+// belongs to it, and zeros there stay zeros.
+template <int BITS>
+__global__ void __launch_bounds__(BLOCK) step_kernel(
+    float* __restrict__ param, const float* __restrict__ grad,
+    float* __restrict__ m32, float* __restrict__ v32,
+    uint2* __restrict__ codes, uchar2* __restrict__ exps,
+    const long* __restrict__ chunks, const float* __restrict__ decay,
+    const float* __restrict__ coef, const long* __restrict__ step,
+    float* __restrict__ part, Hyper h) {
+  const long start = chunks[3 * blockIdx.x];
+  const int len = (int)chunks[3 * blockIdx.x + 1];
+  const float wd = decay[chunks[3 * blockIdx.x + 2]];
+  const float lr = coef[0], k1 = coef[1], k2 = coef[2];
+  const unsigned key = hash_u32(h.seed, (unsigned)(step[0] + 1));
+  const int padded = (len + QB - 1) / QB * QB;
+  float acc = 0.f;
+  for (int i = threadIdx.x * 4; i < padded; i += BLOCK * 4) {
+    const long at = start + i;
+    float4 p = *reinterpret_cast<const float4*>(param + at);
+    const float4 g = *reinterpret_cast<const float4*>(grad + at);
+    float4 m, v;
+    float* pp = reinterpret_cast<float*>(&p);
+    const float* gg = reinterpret_cast<const float*>(&g);
+    float* mm = reinterpret_cast<float*>(&m);
+    float* vv = reinterpret_cast<float*>(&v);
+    if (BITS == 32) {
+      m = *reinterpret_cast<const float4*>(m32 + at);
+      v = *reinterpret_cast<const float4*>(v32 + at);
+    } else {
+      const uint2 code = codes[at >> 2];
+      const uchar2 e = exps[at / QB];
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        mm[j] = decode_m((code.x >> (8 * j)) & 255u, e.x);
+        vv[j] = decode_v((code.y >> (8 * j)) & 255u, e.y);
+      }
+    }
+    unsigned top_m = 0, top_v = 0;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      mm[j] = ema(mm[j], h.b1, gg[j], h.c1);
+      vv[j] = ema(vv[j], h.b2, square(gg[j]), h.c2);
+      pp[j] = stepped(pp[j], mm[j], vv[j], lr, k1, k2, h.eps, wd);
+      if (i + j < len) acc = fmaf(pp[j], pp[j], acc);
+      top_m = max(top_m, __float_as_uint(mm[j]) & 0x7fffffffu);
+      top_v = max(top_v, __float_as_uint(vv[j]) & 0x7fffffffu);
+    }
+    *reinterpret_cast<float4*>(param + at) = p;
+    if (BITS == 32) {
+      *reinterpret_cast<float4*>(m32 + at) = m;
+      *reinterpret_cast<float4*>(v32 + at) = v;
+    } else {
+      // 16 lanes hold one block of 64, and all of them are here: chunks are
+      // cut and padded in whole blocks
+      const int em = shared_exponent<4>(max16(top_m));
+      const int ev = shared_exponent<5>(max16(top_v));
+      uint2 code = {0u, 0u};
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const unsigned long place = (unsigned long)(at + j);
+        const unsigned r =
+            hash_u32(key + (unsigned)(place >> 32), (unsigned)place);
+        unsigned qm = encode<4>(mm[j], em, r & 0xffffu);
+        qm |= (__float_as_uint(mm[j]) >> 31) << 7;
+        unsigned qv = encode<5>(vv[j], ev, r >> 16);
+        if (qv == 0 && vv[j] > 0.f) qv = 1;
+        code.x |= qm << (8 * j);
+        code.y |= qv << (8 * j);
+      }
+      codes[at >> 2] = code;
+      if ((threadIdx.x & 15) == 0)
+        exps[at / QB] = make_uchar2((unsigned char)em, (unsigned char)ev);
+    }
+  }
+#pragma unroll
+  for (int d = 32; d; d >>= 1) acc += __shfl_xor(acc, d);
+  __shared__ float waves[BLOCK / 64];
+  if ((threadIdx.x & 63) == 0) waves[threadIdx.x >> 6] = acc;
+  __syncthreads();
+  if (threadIdx.x == 0) {
+    float s = 0.f;
+    for (int w = 0; w < BLOCK / 64; ++w) s += waves[w];
+    part[blockIdx.x] = s;
+  }
+}
+
+// one wave a tensor: its chunks' parts, added in a fixed order. The first
+// block moves the step on.
+__global__ void __launch_bounds__(64) finish_kernel(
+    const float* __restrict__ part, const long* __restrict__ first,
+    float* __restrict__ norms, float* __restrict__ coef,
+    long* __restrict__ step, double b1, double b2) {
+  const long a = first[blockIdx.x], b = first[blockIdx.x + 1];
+  float acc = 0.f;
+  for (long i = a + threadIdx.x; i < b; i += 64) acc += part[i];
+#pragma unroll
+  for (int d = 32; d; d >>= 1) acc += __shfl_xor(acc, d);
+  if (threadIdx.x == 0) {
+    norms[blockIdx.x] = acc;
+    if (blockIdx.x == 0) {
+      const long t = step[0] + 1;
+      step[0] = t;
+      coef[1] = (float)(1.0 / (1.0 - pow(b1, (double)(t + 1))));
+      coef[2] = (float)(1.0 / sqrt(1.0 - pow(b2, (double)(t + 1))));
+    }
+  }
+}
+
+__global__ void __launch_bounds__(BLOCK) moments_kernel(
+    const uint2* __restrict__ codes, const uchar2* __restrict__ exps,
+    bf16x4* __restrict__ m, bf16x4* __restrict__ v, long quads) {
+  const long stride = (long)gridDim.x * BLOCK;
+  for (long i = (long)blockIdx.x * BLOCK + threadIdx.x; i < quads;
+       i += stride) {
+    const uint2 code = codes[i];
+    const uchar2 e = exps[i / (QB / 4)];
+    bf16x4 a, b;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      a[j] = (__bf16)decode_m((code.x >> (8 * j)) & 255u, e.x);
+      b[j] = (__bf16)decode_v((code.y >> (8 * j)) & 255u, e.y);
+    }
+    m[i] = a;
+    v[i] = b;
+  }
+}
+
+static void check(const torch::Tensor& t, const char* name,
+                  c10::ScalarType type, long numel,
+                  const torch::Tensor& like) {
+  TORCH_CHECK(t.is_cuda() && t.device() == like.device(), name,
+              " must be on the parameters' GPU");
+  TORCH_CHECK(t.is_contiguous(), name, " must be contiguous");
+  TORCH_CHECK(t.scalar_type() == type, name, " must be ", type, ", got ",
+              t.scalar_type());
+  TORCH_CHECK(t.numel() == numel, name, " must have ", numel,
+              " elements, got ", t.numel());
+}
+
+}  // namespace adamw
+
+// codes: for each 4 values 4 bytes of m, then 4 of v; exps: for each 64 the
+// exponents of m and of v. Where they are empty the moments are m and v in
+// fp32. chunks [k, 3] lists each tensor's chunks in turn, first[i] is the
+// place of tensor i's first chunk; both are the caller's plan, made for
+// param's layout.
+torch::Tensor adamw_step_norm(torch::Tensor param, torch::Tensor grad,
+                              torch::Tensor m, torch::Tensor v,
+                              torch::Tensor codes, torch::Tensor exps,
+                              torch::Tensor chunks, torch::Tensor first,
+                              torch::Tensor decay, torch::Tensor coef,
+                              torch::Tensor step, double b1, double b2,
+                              double eps, long seed) {
+  using namespace adamw;
+  CHECK_IN(param);
+  TORCH_CHECK(param.scalar_type() == torch::kFloat32, "param must be fp32");
+  const long n = param.numel();
+  TORCH_CHECK(n % QB == 0, "the flat space must be padded to ", QB);
+  TORCH_CHECK((reinterpret_cast<uintptr_t>(param.data_ptr()) |
+               reinterpret_cast<uintptr_t>(grad.data_ptr())) % 16 == 0,
+              "param and grad must be 16-byte aligned");
+  const bool bits8 = codes.numel() > 0;
+  check(grad, "grad", torch::kFloat32, n, param);
+  if (bits8) {
+    check(codes, "codes", torch::kUInt8, 2 * n, param);
+    check(exps, "exps", torch::kUInt8, 2 * (n / QB), param);
+  } else {
+    check(m, "m", torch::kFloat32, n, param);
+    check(v, "v", torch::kFloat32, n, param);
+  }
+  const long sz = decay.numel(), k = chunks.numel() / 3;
+  check(chunks, "chunks", torch::kInt64, 3 * k, param);
+  check(first, "first", torch::kInt64, sz + 1, param);
+  check(decay, "decay", torch::kFloat32, sz, param);
+  check(coef, "coef", torch::kFloat32, 3, param);
+  check(step, "step", torch::kInt64, 1, param);
+  const c10::DeviceGuard guard(param.device());
+  auto norms = torch::empty({sz}, param.options());
+  if (sz == 0) return norms;
+  auto part = torch::empty({k}, param.options());
+  const Hyper h{(float)b1, (float)(1.0 - b1), (float)b2, (float)(1.0 - b2),
+                (float)eps, (unsigned)seed};
+  auto run = [&](auto kernel) {
+    kernel<<<(unsigned)k, BLOCK, 0, cur_stream()>>>(
+        param.data_ptr<float>(), grad.data_ptr<float>(),
+        bits8 ? nullptr : m.data_ptr<float>(),
+        bits8 ? nullptr : v.data_ptr<float>(),
+        bits8 ? reinterpret_cast<uint2*>(codes.data_ptr()) : nullptr,
+        bits8 ? reinterpret_cast<uchar2*>(exps.data_ptr()) : nullptr,
+        chunks.data_ptr<long>(), decay.data_ptr<float>(),
+        coef.data_ptr<float>(), step.data_ptr<long>(),
+        part.data_ptr<float>(), h);
+  };
+  if (k) {
+    if (bits8) run(step_kernel<8>); else run(step_kernel<32>);
+  }
+  finish_kernel<<<(unsigned)sz, 64, 0, cur_stream()>>>(
+      part.data_ptr<float>(), first.data_ptr<long>(),
+      norms.data_ptr<float>(), coef.data_ptr<float>(), step.data_ptr<long>(),
+      b1, b2);
+  return norms;
+}
+
+// the values that 8-bit moments stand for, exact in bfloat16
+std::vector<torch::Tensor> adamw_moments(torch::Tensor codes,
+                                         torch::Tensor exps) {
+  using namespace adamw;
+  CHECK_IN(codes);
+  const long n = codes.numel() / 2;
+  TORCH_CHECK(n % QB == 0 && codes.numel() == 2 * n, "codes must hold whole "
+              "blocks of ", QB);
+  check(codes, "codes", torch::kUInt8, 2 * n, codes);
+  check(exps, "exps", torch::kUInt8, 2 * (n / QB), codes);
+  const c10::DeviceGuard guard(codes.device());
+  auto m = torch::empty({n}, codes.options().dtype(torch::kBFloat16));
+  auto v = torch::empty_like(m);
+  if (n == 0) return {m, v};
+  const long quads = n / 4;
+  const int grid = (int)std::min<long>((quads + BLOCK - 1) / BLOCK, 4096L);
+  moments_kernel<<<grid, BLOCK, 0, cur_stream()>>>(
+      reinterpret_cast<const uint2*>(codes.data_ptr()),
+      reinterpret_cast<const uchar2*>(exps.data_ptr()),
+      reinterpret_cast<bf16x4*>(m.data_ptr()),
+      reinterpret_cast<bf16x4*>(v.data_ptr()), quads);
+  return {m, v};
+}
+
+}  // namespace eg

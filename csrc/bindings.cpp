@@ -19,6 +19,13 @@ torch::Tensor trigger_update(torch::Tensor, torch::Tensor, torch::Tensor,
                              long, bool, double, double, long, bool);
 torch::Tensor trigger_decide(torch::Tensor, torch::Tensor, torch::Tensor,
                              long, bool, double, double, long);
+// adamw.hip
+torch::Tensor adamw_step_norm(torch::Tensor, torch::Tensor, torch::Tensor,
+                              torch::Tensor, torch::Tensor, torch::Tensor,
+                              torch::Tensor, torch::Tensor, torch::Tensor,
+                              torch::Tensor, torch::Tensor, double, double,
+                              double, long);
+std::vector<torch::Tensor> adamw_moments(torch::Tensor, torch::Tensor);
 // elementwise.hip
 torch::Tensor relu_fwd(torch::Tensor);
 torch::Tensor relu_bwd(torch::Tensor, torch::Tensor);
@@ -65,6 +72,14 @@ std::vector<torch::Tensor> bn_stats_finalize(torch::Tensor, torch::Tensor,
                                              bool);
 torch::Tensor bn_norm_add_relu(torch::Tensor, torch::Tensor, torch::Tensor,
                                torch::Tensor, torch::Tensor, torch::Tensor);
+// groupnorm.hip
+std::vector<torch::Tensor> group_norm_fwd(torch::Tensor, torch::Tensor,
+                                          torch::Tensor, long, double, long,
+                                          c10::optional<torch::Tensor>);
+std::vector<torch::Tensor> group_norm_bwd(
+    torch::Tensor, torch::Tensor, torch::Tensor, torch::Tensor, torch::Tensor,
+    long, long, c10::optional<torch::Tensor>, bool, bool,
+    c10::optional<torch::Tensor>, c10::optional<torch::Tensor>);
 // pool.hip
 std::vector<torch::Tensor> maxpool2x2_fwd(torch::Tensor);
 torch::Tensor maxpool2x2_bwd(torch::Tensor, torch::Tensor, long, long);
@@ -92,6 +107,8 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.def("scatter_segments", &eg::scatter_segments);
   m.def("trigger_update", &eg::trigger_update);
   m.def("trigger_decide", &eg::trigger_decide);
+  m.def("adamw_step_norm", &eg::adamw_step_norm);
+  m.def("adamw_moments", &eg::adamw_moments);
   m.def("relu_fwd", &eg::relu_fwd);
   m.def("relu_bwd", &eg::relu_bwd);
   m.def("add_relu_fwd", &eg::add_relu_fwd);
@@ -129,6 +146,15 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.def("relu_bwd_bnstats", &eg::relu_bwd_bnstats);
   m.def("bn_stats_finalize", &eg::bn_stats_finalize);
   m.def("bn_norm_add_relu", &eg::bn_norm_add_relu);
+  m.def("group_norm_fwd", &eg::group_norm_fwd, py::arg("x"), py::arg("gamma"),
+        py::arg("beta"), py::arg("groups"), py::arg("eps"), py::arg("act"),
+        py::arg("residual") = c10::nullopt);
+  m.def("group_norm_bwd", &eg::group_norm_bwd, py::arg("dy"), py::arg("x"),
+        py::arg("stats"), py::arg("gamma"), py::arg("beta"),
+        py::arg("groups"), py::arg("act"), py::arg("residual"),
+        py::arg("want_dx"), py::arg("want_dres"),
+        py::arg("dgamma_out") = c10::nullopt,
+        py::arg("dbeta_out") = c10::nullopt);
   m.def("maxpool2x2_fwd", &eg::maxpool2x2_fwd);
   m.def("maxpool2x2_bwd", &eg::maxpool2x2_bwd);
   m.def("avgpool_fwd", &eg::avgpool_fwd);

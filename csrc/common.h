@@ -33,15 +33,19 @@ static inline int ceil_div(long a, long b) { return (int)((a + b - 1) / b); }
 // defined in bn.hip; used by conv.hip's fused-BN-stats epilogue
 float* bn_stats_ws_ptr(int c, torch::TensorOptions opts);
 
-// simple per-element hash RNG (wang hash), uniform in [0,1)
-__device__ __forceinline__ float hash_uniform(unsigned seed, unsigned idx) {
+// simple per-element hash RNG (wang hash): 32 bits
+__device__ __forceinline__ unsigned hash_u32(unsigned seed, unsigned idx) {
   unsigned h = seed ^ (idx * 0x9E3779B9u);
   h = (h ^ 61u) ^ (h >> 16);
   h *= 9u;
   h = h ^ (h >> 4);
   h *= 0x27d4eb2du;
-  h = h ^ (h >> 15);
-  return (h & 0x00FFFFFFu) * (1.0f / 16777216.0f);
+  return h ^ (h >> 15);
+}
+
+// uniform in [0,1)
+__device__ __forceinline__ float hash_uniform(unsigned seed, unsigned idx) {
+  return (hash_u32(seed, idx) & 0x00FFFFFFu) * (1.0f / 16777216.0f);
 }
 
 }  // namespace eg

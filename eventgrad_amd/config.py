@@ -46,13 +46,23 @@ class TriggerConfig:
 
 @dataclass
 class OptimConfig:
-    """Plain/momentum SGD (the only optimizer the reference uses)."""
+    """Plain/momentum SGD (the only optimizer the reference uses), or AdamW.
+
+    momentum is SGD's alone; beta1 to state_bits are AdamW's. weight_decay
+    is added to the gradient by SGD and taken off the weights by AdamW.
+    """
 
     lr: float = 0.01
     momentum: float = 0.0
     weight_decay: float = 0.0
     # divide allreduced gradients by world size in cent mode (cent.cpp:140)
     average_grads: bool = True
+    optimizer: str = "sgd"        # sgd | adamw
+    beta1: float = 0.9
+    beta2: float = 0.999
+    eps: float = 1e-8
+    decay_1d: bool = True         # decay biases and norm weights too
+    state_bits: int = 32          # bits of each moment: 32 | 8
 
 
 @dataclass
@@ -108,6 +118,9 @@ class RunConfig:
     # evaluation
     eval_at_end: bool = True
     final_consensus: bool = True  # closing param AllReduce (event.cpp:517-525)
+    # the ResNets' norm layers: batch | group (of norm_groups groups)
+    norm: str = "batch"
+    norm_groups: int = 8
 
     def to_json(self) -> str:
         return json.dumps(dataclasses.asdict(self), indent=2)

@@ -10,16 +10,23 @@
   - resnetN   standard ResNets (layers[i] blocks per stage)
 """
 
-from .layers import Conv2d, BatchNorm2d, Linear  # noqa: F401
+from .layers import (Conv2d, BatchNorm2d, GroupNorm2d, Linear,  # noqa: F401
+                     norm_factory)
 from .mlp import MLP  # noqa: F401
 from .cnn import CNN1, CNN2, LeNet5  # noqa: F401
 from .resnet import ResNet, BasicBlock, BottleNeck  # noqa: F401
 
 
-def build_model(name: str, num_classes: int = 10):
+def build_model(name: str, num_classes: int = 10, norm: str = "batch",
+                norm_groups: int = 8):
+    """norm: what follows each conv of a ResNet, "batch" or "group" (of
+    `norm_groups` groups); the other models have no norms."""
     from .resnet import resnet_factory
 
     name = name.lower()
+    layer = norm_factory(norm, norm_groups)
+    if norm != "batch" and not name.startswith("resnet"):
+        raise ValueError(f"model {name!r} has no norm layers")
     if name == "mlp":
         return MLP()
     if name == "cnn1":
@@ -29,7 +36,7 @@ def build_model(name: str, num_classes: int = 10):
     if name == "lenet5":
         return LeNet5()
     if name.startswith("resnet"):
-        return resnet_factory(name, num_classes)
+        return resnet_factory(name, num_classes, layer)
     raise ValueError(f"unknown model {name!r}")
 
 

@@ -11,6 +11,7 @@ are never communicated (SURVEY.md §2.6 note on BatchNorm2d).
 
 from __future__ import annotations
 
+import functools
 import math
 
 import torch
@@ -55,6 +56,8 @@ class Conv2d(nn.Module):
 
 
 class BatchNorm2d(nn.Module):
+    batch_statistics = True  # a conv's epilogue can collect them
+
     def __init__(self, num_features, eps=1e-5, momentum=0.1):
         super().__init__()
         self.num_features, self.eps, self.momentum = num_features, eps, momentum
@@ -91,6 +94,48 @@ class BatchNorm2d(nn.Module):
                             stats_ready and O.use_native(x) and self.training
                             and self.num_features % 64 == 0,
                             stash_module=self if stats_consumer else None)
+
+
+class GroupNorm2d(nn.Module):
+    """Group norm, with the activation and the residual in the same pass.
+
+    It has no running statistics: all of it is parameters, which the gossip
+    averages, and it does not depend on the per-rank batch."""
+
+    batch_statistics = False
+
+    def __init__(self, num_features, groups=8, eps=1e-5):
+        super().__init__()
+        if groups < 1 or num_features % groups:
+            raise ValueError(f"{num_features} channels do not divide into "
+                             f"{groups} groups")
+        self.num_features, self.groups, self.eps = num_features, groups, eps
+        self.weight = nn.Parameter(torch.ones(num_features))
+        self.bias = nn.Parameter(torch.zeros(num_features))
+
+    def forward(self, x, activation: str = "none", residual=None):
+        return O.group_norm(x, self.weight, self.bias, self.groups, self.eps,
+                            activation, residual)
+
+    def extra_repr(self):
+        return f"{self.num_features}, groups={self.groups}"
+
+
+def norm_factory(norm: str = "batch", groups: int = 8):
+    """The norm layer that a model puts behind each conv: channels -> module.
+    norm: "batch" or "group" (of `groups` groups)."""
+    if norm == "batch":
+        return BatchNorm2d
+    if norm == "group":
+        return functools.partial(GroupNorm2d, groups=groups)
+    raise ValueError(f"norm must be 'batch' or 'group', got {norm!r}")
+
+
+def conv_norm(conv, norm, x, relu: bool = False):
+    """norm(conv(x)), with a ReLU behind it where asked."""
+    if not norm.batch_statistics:
+        return norm(conv(x), activation="relu" if relu else "none")
+    return norm(conv(x, bn_stats=True), fuse_relu=relu, stats_ready=True)
 
 
 class Linear(nn.Module):

@@ -14,6 +14,10 @@ blocks, 17,444,682 parameters in 86 named tensors. We keep
 that behaviour under the ``quirk=True`` models (``resnet18q`` — the
 configuration the reference's CIFAR-10 baselines and message counts are
 quoted on) and also provide standard counts (``resnet18``).
+
+Every conv is followed by a norm: batch norm, as in the reference, or group
+norm (``norm_factory``), which keeps no statistics outside the parameters that
+the ranks exchange.
 """
 
 from __future__ import annotations
@@ -21,7 +25,7 @@ from __future__ import annotations
 from torch import nn
 
 from ..ops import functional as O
-from .layers import BatchNorm2d, Conv2d
+from .layers import BatchNorm2d, Conv2d, conv_norm
 
 
 def conv_op(in_ch, out_ch, k, stride, padding):
@@ -30,30 +34,38 @@ def conv_op(in_ch, out_ch, k, stride, padding):
 
 
 class Downsampler(nn.Module):
-    """1x1 conv + BN shortcut (resnet.hpp:166-171)."""
+    """1x1 conv + norm shortcut (resnet.hpp:166-171)."""
 
-    def __init__(self, in_ch, out_ch, stride):
+    def __init__(self, in_ch, out_ch, stride, norm=BatchNorm2d):
         super().__init__()
         self.conv = conv_op(in_ch, out_ch, 1, stride, 0)
-        self.bn = BatchNorm2d(out_ch)
+        self.bn = norm(out_ch)
 
     def forward(self, x):
-        return self.bn(self.conv(x, bn_stats=True), stats_ready=True)
+        return conv_norm(self.conv, self.bn, x)
 
 
 class BasicBlock(nn.Module):
     expansion = 1
 
-    def __init__(self, in_ch, out_ch, stride=1, downsample: bool = False):
+    def __init__(self, in_ch, out_ch, stride=1, downsample: bool = False,
+                 norm=BatchNorm2d):
         super().__init__()
         self.conv1 = conv_op(in_ch, out_ch, 3, stride, 1)
-        self.bn1 = BatchNorm2d(out_ch)
+        self.bn1 = norm(out_ch)
         self.conv2 = conv_op(out_ch, out_ch, 3, 1, 1)
-        self.bn2 = BatchNorm2d(out_ch)
-        self.downsampler = (Downsampler(in_ch, out_ch * self.expansion, stride)
+        self.bn2 = norm(out_ch)
+        self.downsampler = (Downsampler(in_ch, out_ch * self.expansion, stride,
+                                        norm)
                             if downsample else None)
 
     def forward(self, x):
+        if not self.bn1.batch_statistics:
+            residual = (self.downsampler(x) if self.downsampler is not None
+                        else x)
+            out = conv_norm(self.conv1, self.bn1, x, relu=True)
+            return self.bn2(self.conv2(out), activation="relu",
+                            residual=residual)
         # bn1 -> conv2 is single-consumer: conv2's dgrad epilogue can
         # accumulate bn1's backward stats (ops/functional.py)
         f1 = O.can_fuse_dgrad_stats(self.bn1, self.conv2, x)
@@ -73,18 +85,27 @@ class BasicBlock(nn.Module):
 class BottleNeck(nn.Module):
     expansion = 4
 
-    def __init__(self, in_ch, out_ch, stride=1, downsample: bool = False):
+    def __init__(self, in_ch, out_ch, stride=1, downsample: bool = False,
+                 norm=BatchNorm2d):
         super().__init__()
         self.conv1 = conv_op(in_ch, out_ch, 1, 1, 0)
-        self.bn1 = BatchNorm2d(out_ch)
+        self.bn1 = norm(out_ch)
         self.conv2 = conv_op(out_ch, out_ch, 3, stride, 1)
-        self.bn2 = BatchNorm2d(out_ch)
+        self.bn2 = norm(out_ch)
         self.conv3 = conv_op(out_ch, out_ch * self.expansion, 1, 1, 0)
-        self.bn3 = BatchNorm2d(out_ch * self.expansion)
-        self.downsampler = (Downsampler(in_ch, out_ch * self.expansion, stride)
+        self.bn3 = norm(out_ch * self.expansion)
+        self.downsampler = (Downsampler(in_ch, out_ch * self.expansion, stride,
+                                        norm)
                             if downsample else None)
 
     def forward(self, x):
+        if not self.bn1.batch_statistics:
+            residual = (self.downsampler(x) if self.downsampler is not None
+                        else x)
+            out = conv_norm(self.conv1, self.bn1, x, relu=True)
+            out = conv_norm(self.conv2, self.bn2, out, relu=True)
+            return self.bn3(self.conv3(out), activation="relu",
+                            residual=residual)
         f1 = O.can_fuse_dgrad_stats(self.bn1, self.conv2, x)
         out = self.bn1(self.conv1(x, bn_stats=True), fuse_relu=True,
                        stats_ready=True, stats_consumer=f1)
@@ -107,11 +128,12 @@ class CifarResNet(nn.Module):
     flagship benchmark uses that quirk model for fidelity.
     """
 
-    def __init__(self, n: int, num_classes: int = 10):
+    def __init__(self, n: int, num_classes: int = 10, norm=BatchNorm2d):
         super().__init__()
         self.in_channels = 16
+        self.norm = norm
         self.conv = conv_op(3, 16, 3, 1, 1)
-        self.bn = BatchNorm2d(16)
+        self.bn = norm(16)
         self.layer1 = self._make_stage(16, n, 1)
         self.layer2 = self._make_stage(32, n, 2)
         self.layer3 = self._make_stage(64, n, 2)
@@ -121,16 +143,16 @@ class CifarResNet(nn.Module):
     def _make_stage(self, out_ch, blocks, stride):
         layers = [BasicBlock(self.in_channels, out_ch, stride,
                              downsample=(stride != 1
-                                         or self.in_channels != out_ch))]
+                                         or self.in_channels != out_ch),
+                             norm=self.norm)]
         self.in_channels = out_ch
         for _ in range(blocks - 1):
-            layers.append(BasicBlock(out_ch, out_ch))
+            layers.append(BasicBlock(out_ch, out_ch, norm=self.norm))
         return nn.Sequential(*layers)
 
     def forward(self, x):
         x = O.to_compute(x)
-        out = self.bn(self.conv(x, bn_stats=True), fuse_relu=True,
-                      stats_ready=True)
+        out = conv_norm(self.conv, self.bn, x, relu=True)
         out = self.layer1(out)
         out = self.layer2(out)
         out = self.layer3(out)
@@ -141,11 +163,13 @@ class CifarResNet(nn.Module):
 
 
 class ResNet(nn.Module):
-    def __init__(self, block, layers, num_classes=10, quirk=True):
+    def __init__(self, block, layers, num_classes=10, quirk=True,
+                 norm=BatchNorm2d):
         super().__init__()
         self.in_channels = 64
+        self.norm = norm
         self.conv = conv_op(3, 64, 3, 1, 1)
-        self.bn = BatchNorm2d(64)
+        self.bn = norm(64)
         self.layer1 = self._make_layer(block, 64, layers[0], 1, quirk)
         self.layer2 = self._make_layer(block, 128, layers[1], 2, quirk)
         self.layer3 = self._make_layer(block, 256, layers[2], 2, quirk)
@@ -157,19 +181,19 @@ class ResNet(nn.Module):
         layers = []
         downsample = (stride != 1
                       or self.in_channels != out_ch * block.expansion)
-        layers.append(block(self.in_channels, out_ch, stride, downsample))
+        layers.append(block(self.in_channels, out_ch, stride, downsample,
+                            norm=self.norm))
         self.in_channels = out_ch * block.expansion
         # reference quirk (resnet.hpp:172-178): `blocks` MORE blocks after the
         # strided one (layers[i]+1 total); standard builds blocks-1 more.
         extra = blocks if quirk else blocks - 1
         for _ in range(extra):
-            layers.append(block(self.in_channels, out_ch))
+            layers.append(block(self.in_channels, out_ch, norm=self.norm))
         return nn.Sequential(*layers)
 
     def forward(self, x):
         x = O.to_compute(x)
-        out = self.bn(self.conv(x, bn_stats=True), fuse_relu=True,
-                      stats_ready=True)
+        out = conv_norm(self.conv, self.bn, x, relu=True)
         out = self.layer1(out)
         out = self.layer2(out)
         out = self.layer3(out)
@@ -189,14 +213,14 @@ _CONFIGS = {
 }
 
 
-def resnet_factory(name: str, num_classes: int = 10):
+def resnet_factory(name: str, num_classes: int = 10, norm=BatchNorm2d):
     # classic CIFAR depths: resnet20/32/44/56 (depth = 6n+2)
     if name in ("resnet20", "resnet32", "resnet44", "resnet56"):
         n = (int(name[6:]) - 2) // 6
-        return CifarResNet(n, num_classes)
+        return CifarResNet(n, num_classes, norm)
     quirk = name.endswith("q")
     base = name[:-1] if quirk else name
     if base not in _CONFIGS:
         raise ValueError(f"unknown resnet {name!r}")
     block, layers = _CONFIGS[base]
-    return ResNet(block, layers, num_classes, quirk=quirk)
+    return ResNet(block, layers, num_classes, quirk=quirk, norm=norm)

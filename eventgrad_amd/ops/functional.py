@@ -244,6 +244,117 @@ def batch_norm(x, gamma, beta, running_mean, running_var, training,
 
 
 # --------------------------------------------------------------------------
+# group norm (+ fused residual and activation)
+# --------------------------------------------------------------------------
+
+_ACTIVATIONS = {"none": 0, "relu": 1, "silu": 2}
+
+
+class _GroupNormNHWC(torch.autograd.Function):
+    """Gradients of gamma and beta go straight into pre-allocated .grad views
+    (added to what is there), like those of the other layers; a standalone
+    parameter gets its gradient from autograd."""
+
+    @staticmethod
+    def forward(ctx, x, gamma, beta, residual, groups, eps, act):
+        y, stats = native().group_norm_fwd(x, gamma.detach(), beta.detach(),
+                                           groups, eps, act, residual)
+        # without an activation the gradient does not need the residual
+        ctx.save_for_backward(x, gamma, beta, stats,
+                              residual if act else None)
+        ctx.groups, ctx.act = groups, act
+        ctx.ggrad = gamma.grad if gamma.requires_grad else None
+        ctx.bgrad = beta.grad if beta.requires_grad else None
+        return y
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, dy):
+        x, gamma, beta, stats, residual = ctx.saved_tensors
+        want_x, want_g, want_b, want_r = ctx.needs_input_grad[:4]
+        dy = dy.contiguous()
+        direct = (want_g and want_b and ctx.ggrad is not None
+                  and ctx.bgrad is not None)
+        dx, dres, dgamma, dbeta = native().group_norm_bwd(
+            dy, x, stats, gamma.detach(), beta.detach(), ctx.groups, ctx.act,
+            residual, want_x, want_r and ctx.act != 0,
+            ctx.ggrad if direct else None, ctx.bgrad if direct else None)
+        if want_r and ctx.act == 0:
+            dres = dy
+        return (dx, dgamma if want_g and not direct else None,
+                dbeta if want_b and not direct else None, dres,
+                None, None, None)
+
+
+def _group_norm_plain(x, gamma, beta, groups, eps, act, residual):
+    n, c = x.shape[:2]
+    if x.numel() == 0:
+        y = x + 0 * (gamma.sum() + beta.sum())
+    else:
+        xg = x.reshape(n, groups, -1)
+        var, mean = torch.var_mean(xg, dim=2, correction=0, keepdim=True)
+        y = ((xg - mean) * torch.rsqrt(var + eps)).reshape(x.shape)
+        y = y * gamma.view(1, c, 1, 1) + beta.view(1, c, 1, 1)
+    if residual is not None:
+        y = y + residual
+    return (y, F.relu(y), F.silu(y))[act] if act else y
+
+
+def group_norm(x, gamma, beta, groups, eps=1e-5, activation="none",
+               residual=None):
+    """act(group_norm(x) * gamma + beta + residual).
+
+    Statistics are taken over each sample's groups of C / groups neighbouring
+    channels; there are no running statistics, and training and evaluation
+    are the same. activation: "none", "relu" or "silu". On the GPU x is
+    [N, H, W, C], contiguous, in bf16 (fp16 and fp32 work too), the residual
+    is like x, and gamma and beta are fp32; the normalisation, the sum and
+    the activation are one pass, and so are their gradients. On the CPU x is
+    [N, C, H, W].
+
+    In a captured region gamma and beta need pre-allocated gradients
+    (FlatParamSpace gives them), and x and the residual must not themselves
+    be leaves that want one: autograd's own accumulation into a leaf that an
+    eager graph also holds cannot be captured.
+    """
+    if activation not in _ACTIVATIONS:
+        raise ValueError(f"activation must be one of "
+                         f"{sorted(_ACTIVATIONS)}, got {activation!r}")
+    if not isinstance(groups, int) or groups < 1:
+        raise ValueError(f"groups must be a positive int, got {groups!r}")
+    if not eps >= 0:
+        raise ValueError(f"eps must not be negative, got {eps!r}")
+    if x.dim() != 4:
+        raise ValueError(f"group_norm takes a 4-d tensor, got {x.dim()}-d")
+    act = _ACTIVATIONS[activation]
+    native_path = use_native(x)
+    c = x.shape[3] if native_path else x.shape[1]
+    if c == 0 or c % groups:
+        raise ValueError(f"{c} channels do not divide into {groups} groups")
+    if residual is not None and residual.shape != x.shape:
+        raise ValueError(f"the residual must have x's shape "
+                         f"{tuple(x.shape)}, got {tuple(residual.shape)}")
+    if not native_path:
+        return _group_norm_plain(x, gamma, beta, groups, eps, act, residual)
+    inputs = (x, gamma, beta) + (() if residual is None else (residual,))
+    if not (torch.is_grad_enabled() and any(t.requires_grad for t in inputs)):
+        return native().group_norm_fwd(x, gamma, beta, groups, eps, act,
+                                       residual)[0]
+    if torch.cuda.is_current_stream_capturing():
+        for t in inputs:
+            param = t is gamma or t is beta
+            if t.requires_grad and t.is_leaf and not (
+                    param and t.grad is not None):
+                raise RuntimeError(
+                    "group_norm: a captured backward pass cannot accumulate "
+                    "into this leaf; give gamma and beta pre-allocated "
+                    "gradients, and make x and the residual in the captured "
+                    "region")
+    return _GroupNormNHWC.apply(x, gamma, beta, residual, groups, float(eps),
+                                act)
+
+
+# --------------------------------------------------------------------------
 # elementwise: relu / residual add+relu / dropout
 # --------------------------------------------------------------------------
 
@@ -322,7 +433,8 @@ class _BnTail(torch.autograd.Function):
 def can_fuse_dgrad_stats(bn, conv, x) -> bool:
     """Eligibility for fusing `bn`'s backward stats into `conv`'s dgrad
     epilogue (bn -> conv single-consumer chain inside a block)."""
-    return (use_native(x) and bn.training
+    return (use_native(x) and getattr(bn, "batch_statistics", True)
+            and bn.training
             and bn.weight.grad is not None and bn.bias.grad is not None
             and bn.num_features % 64 == 0
             and conv.stride == 1 and conv.out_ch % 8 == 0

@@ -22,5 +22,6 @@ Mapping from the reference's MPI call sites:
 
 from .dist import init_distributed, ring_neighbors, world_info  # noqa: F401
 from .flat import FlatParamSpace  # noqa: F401
+from .adamw import AdamW  # noqa: F401
 from .controller import TriggerController  # noqa: F401
 from .engine import build_engine  # noqa: F401

@@ -8,7 +8,7 @@ Per-iteration contract with the trainer (pass_num counts from 1):
     engine.after_backward()       # cent: fused-grad allreduce (+ /world);
                                   # gossip: wait transfers, unpack inboxes,
                                   # theta <- (theta + left + right)/3
-    engine.step()                 # fused SGD step + per-tensor L2 norms
+    engine.step()                 # fused SGD or AdamW step + per-tensor norms
     ...
     engine.finalize()             # closing consensus allreduce on params
                                   # (event.cpp:517-525) + num_events reduce
@@ -30,6 +30,7 @@ import torch.distributed as dist
 
 from ..config import RunConfig
 from ..ops.backend import native
+from .adamw import AdamW
 from .controller import TriggerController
 from .flat import FlatParamSpace
 from .transport import RingTransport
@@ -121,6 +122,19 @@ class _GpuK:
         native().scatter_segments(payload, dst, offs, inbox)
 
 
+def _build_adamw(space, cfg: RunConfig):
+    """The AdamW of a run; None where SGD steps (state: space.momentum)."""
+    o = cfg.optim
+    if o.optimizer == "sgd":
+        return None
+    if o.optimizer != "adamw":
+        raise ValueError(f"optimizer must be 'sgd' or 'adamw', "
+                         f"got {o.optimizer!r}")
+    return AdamW(space, lr=o.lr, betas=(o.beta1, o.beta2), eps=o.eps,
+                 weight_decay=o.weight_decay, decay_1d=o.decay_1d,
+                 state_bits=o.state_bits, seed=cfg.seed)
+
+
 def _kernels(device: torch.device):
     return _GpuK if device.type == "cuda" else _CpuK
 
@@ -137,6 +151,7 @@ class CommEngine:
         self.rank, self.world = rank, world
         self.device = device
         self.K = _kernels(device)
+        self.opt = _build_adamw(space, cfg)
         self.tracer = tracer
         self.pass_num = 0
 
@@ -166,8 +181,13 @@ class CommEngine:
 
     def step(self) -> None:
         o = self.cfg.optim
-        self._last_norms_sq = self.K.sgd_step(self.space, o.lr, o.momentum,
-                                              o.weight_decay)
+        if self.opt is not None:
+            if self.opt.lr != o.lr:
+                self.opt.lr = o.lr
+            self._last_norms_sq = self.opt.step()
+        else:
+            self._last_norms_sq = self.K.sgd_step(self.space, o.lr,
+                                                  o.momentum, o.weight_decay)
         # the step is the last param mutation of a pass: regenerate the
         # bf16 weight shadows the next forward/backward will read
         self.space.refresh_shadows()

@@ -29,7 +29,9 @@ ALIGN = 64  # floats
 
 
 class FlatParamSpace:
-    def __init__(self, model: nn.Module, device: torch.device):
+    def __init__(self, model: nn.Module, device: torch.device,
+                 momentum: bool = True):
+        """momentum: whether SGD's buffer is kept (AdamW has its own)."""
         self.device = device
         self.names: List[str] = []
         shapes = []
@@ -55,7 +57,7 @@ class FlatParamSpace:
 
         self.param = torch.zeros(self.total, dtype=torch.float32, device=device)
         self.grad = torch.zeros_like(self.param)
-        self.momentum = torch.zeros_like(self.param)
+        self.momentum = torch.zeros_like(self.param) if momentum else None
 
         # device-side segment tables for the HIP kernels
         self.starts_t = torch.tensor(starts, dtype=torch.int64, device=device)

@@ -1,6 +1,6 @@
 """Checkpoint / resume (new capability; the reference has none — SURVEY.md §5).
 
-Persists, per rank: flat params, SGD momentum, model buffers (BatchNorm
+Persists, per rank: flat params, SGD momentum or AdamW moments, model buffers (BatchNorm
 running_mean/running_var — registered buffers are NOT named_parameters and
 so live outside FlatParamSpace, resnet.hpp:18-19), pass_num/epoch, the
 trigger controller state (thres / last_sent_norm / last_sent_iter / slopes /
@@ -36,12 +36,15 @@ def save_checkpoint(path: str, cfg, epoch: int, pass_num: int, space, engine,
         "epoch": epoch,
         "pass_num": pass_num,
         "param": space.param.detach().cpu(),
-        "momentum": space.momentum.detach().cpu(),
         "names": space.names,
         "rng_cpu": torch.get_rng_state(),
         "engine": engine_state_dict(engine),
         "extra": extra or {},
     }
+    if space.momentum is not None:
+        state["momentum"] = space.momentum.detach().cpu()
+    if getattr(engine, "opt", None) is not None:
+        state["optimizer"] = engine.opt.state_dict()
     if model is not None:
         # non-parameter state: BN running stats + num_batches_tracked
         for m in model.modules():
@@ -72,8 +75,16 @@ def engine_state_dict(engine) -> dict:
 
 def load_checkpoint(path: str, space, engine, device, model=None) -> dict:
     state = torch.load(path, map_location="cpu", weights_only=False)
+    opt = getattr(engine, "opt", None)
+    if (opt is not None) != ("optimizer" in state):
+        raise ValueError(
+            f"{path} holds the state of {'AdamW' if opt is None else 'SGD'}, "
+            "and this run steps with the other")
+    if opt is not None:
+        opt.load_state_dict(state["optimizer"])
+    elif space.momentum is not None:
+        space.momentum.copy_(state["momentum"].to(device))
     space.param.copy_(state["param"].to(device))
-    space.momentum.copy_(state["momentum"].to(device))
     if model is not None and "buffers" in state:
         bufs = dict(model.named_buffers())
         for name, saved in state["buffers"].items():

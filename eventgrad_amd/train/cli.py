@@ -34,6 +34,13 @@ def build_parser() -> argparse.ArgumentParser:
                    help="synthetic dataset train size (no-network runs)")
     p.add_argument("--lr", type=float, default=None)
     p.add_argument("--momentum", type=float, default=None)
+    p.add_argument("--weight-decay", type=float, default=None)
+    p.add_argument("--optimizer", choices=["sgd", "adamw"], default=None)
+    p.add_argument("--state-bits", type=int, choices=[8, 32], default=None,
+                   help="bits of each of AdamW's moments")
+    p.add_argument("--norm", choices=["batch", "group"], default=None,
+                   help="the ResNets' norm layers")
+    p.add_argument("--norm-groups", type=int, default=None)
     p.add_argument("--seed", type=int, default=None)
     # trigger
     p.add_argument("--thres-adaptive", action="store_true", default=None)
@@ -66,7 +73,8 @@ def config_from_args(args) -> RunConfig:
                        ("epochs", "epochs"), ("seed", "seed"),
                        ("device", "device"),
                        ("checkpoint_path", "checkpoint_path"),
-                       ("trace_dir", "trace_dir")]:
+                       ("trace_dir", "trace_dir"), ("norm", "norm"),
+                       ("norm_groups", "norm_groups")]:
         v = getattr(args, name)
         if v is not None:
             setattr(cfg, attr, v)
@@ -97,6 +105,12 @@ def config_from_args(args) -> RunConfig:
         cfg.optim.lr = args.lr
     if args.momentum is not None:
         cfg.optim.momentum = args.momentum
+    if args.weight_decay is not None:
+        cfg.optim.weight_decay = args.weight_decay
+    if args.optimizer is not None:
+        cfg.optim.optimizer = args.optimizer
+    if args.state_bits is not None:
+        cfg.optim.state_bits = args.state_bits
     if args.thres_constant is not None:
         cfg.trigger.adaptive = False
         cfg.trigger.constant = args.thres_constant

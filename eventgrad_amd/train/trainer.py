@@ -2,7 +2,7 @@
 
 Skeleton: epoch loop -> batch loop -> [comm begin_pass] ->
 zero_grad -> forward -> loss -> backward -> [comm after_backward: allreduce
-or wait+unpack+average] -> fused SGD step (+ per-tensor norms) -> accuracy;
+or wait+unpack+average] -> fused optimizer step (+ per-tensor norms) -> accuracy;
 then final consensus allreduce + event-count reduction + rank-0 test eval.
 """
 
@@ -35,9 +35,11 @@ class Trainer:
         O.set_compute_dtype(cfg.compute_dtype)
         torch.manual_seed(cfg.seed)  # ref: torch::manual_seed(0) everywhere
 
-        self.model = build_model(cfg.model, cfg.data.num_classes)
+        self.model = build_model(cfg.model, cfg.data.num_classes,
+                                 cfg.norm, cfg.norm_groups)
         self.model.to(self.device)
-        self.space = FlatParamSpace(self.model, self.device)
+        self.space = FlatParamSpace(self.model, self.device,
+                                    momentum=cfg.optim.optimizer == "sgd")
 
         self.tracer = Tracer(self.rank, cfg.trace_dir) if cfg.trace else None
         self.engine = build_engine(self.space, cfg, self.rank, self.world,

@@ -21,6 +21,8 @@ SRC = [
     "csrc/gemm.hip",
     "csrc/conv.hip",
     "csrc/bn.hip",
+    "csrc/groupnorm.hip",
+    "csrc/adamw.hip",
     "csrc/pool.hip",
     "csrc/loss.hip",
     "csrc/topk.hip",
