@@ -72,14 +72,9 @@ std::vector<torch::Tensor> bn_stats_finalize(torch::Tensor, torch::Tensor,
                                              bool);
 torch::Tensor bn_norm_add_relu(torch::Tensor, torch::Tensor, torch::Tensor,
                                torch::Tensor, torch::Tensor, torch::Tensor);
-// groupnorm.hip
-std::vector<torch::Tensor> group_norm_fwd(torch::Tensor, torch::Tensor,
-                                          torch::Tensor, long, double, long,
-                                          c10::optional<torch::Tensor>);
-std::vector<torch::Tensor> group_norm_bwd(
-    torch::Tensor, torch::Tensor, torch::Tensor, torch::Tensor, torch::Tensor,
-    long, long, c10::optional<torch::Tensor>, bool, bool,
-    c10::optional<torch::Tensor>, c10::optional<torch::Tensor>);
+// groupnorm_autograd.cpp
+torch::Tensor group_norm(torch::Tensor, torch::Tensor, torch::Tensor,
+                         c10::optional<torch::Tensor>, long, double, long);
 // pool.hip
 std::vector<torch::Tensor> maxpool2x2_fwd(torch::Tensor);
 torch::Tensor maxpool2x2_bwd(torch::Tensor, torch::Tensor, long, long);
@@ -146,15 +141,7 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.def("relu_bwd_bnstats", &eg::relu_bwd_bnstats);
   m.def("bn_stats_finalize", &eg::bn_stats_finalize);
   m.def("bn_norm_add_relu", &eg::bn_norm_add_relu);
-  m.def("group_norm_fwd", &eg::group_norm_fwd, py::arg("x"), py::arg("gamma"),
-        py::arg("beta"), py::arg("groups"), py::arg("eps"), py::arg("act"),
-        py::arg("residual") = c10::nullopt);
-  m.def("group_norm_bwd", &eg::group_norm_bwd, py::arg("dy"), py::arg("x"),
-        py::arg("stats"), py::arg("gamma"), py::arg("beta"),
-        py::arg("groups"), py::arg("act"), py::arg("residual"),
-        py::arg("want_dx"), py::arg("want_dres"),
-        py::arg("dgamma_out") = c10::nullopt,
-        py::arg("dbeta_out") = c10::nullopt);
+  m.def("group_norm", &eg::group_norm);
   m.def("maxpool2x2_fwd", &eg::maxpool2x2_fwd);
   m.def("maxpool2x2_bwd", &eg::maxpool2x2_bwd);
   m.def("avgpool_fwd", &eg::avgpool_fwd);

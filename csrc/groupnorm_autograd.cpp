@@ -1,0 +1,135 @@
+// Group norm's node in autograd. It is C++ and not a Python function because
+// the smallest calls are all launch: a backward pass that has to come back to
+// Python's thread costs more than its kernels.
+#include <torch/csrc/autograd/functions/basic_ops.h>
+#include <torch/extension.h>
+
+#include <c10/hip/HIPGraphsC10Utils.h>
+
+#include <vector>
+
+namespace eg {
+
+std::vector<torch::Tensor> group_norm_fwd(torch::Tensor, torch::Tensor,
+                                          torch::Tensor, long, double, long,
+                                          c10::optional<torch::Tensor>);
+torch::Tensor group_norm_only(torch::Tensor, torch::Tensor, torch::Tensor,
+                              long, double, long,
+                              c10::optional<torch::Tensor>);
+std::vector<torch::Tensor> group_norm_bwd(
+    torch::Tensor, torch::Tensor, torch::Tensor, torch::Tensor, torch::Tensor,
+    long, long, c10::optional<torch::Tensor>, bool, bool,
+    c10::optional<torch::Tensor>, c10::optional<torch::Tensor>);
+
+namespace {
+
+using torch::autograd::AutogradContext;
+using torch::autograd::Variable;
+using torch::autograd::variable_list;
+
+c10::optional<torch::Tensor> if_defined(const torch::Tensor& t) {
+  return t.defined() ? c10::optional<torch::Tensor>(t) : c10::nullopt;
+}
+
+// a result that raises where it is differentiated again
+torch::Tensor once(const torch::Tensor& t) {
+  auto fake = t.detach();
+  fake.set_requires_grad(true);
+  auto node = std::make_shared<torch::autograd::DelayedError>(
+      "group_norm has no second derivative", 1);
+  return (*node)({fake})[0];
+}
+
+// Gradients of gamma and beta go straight into pre-allocated .grad views
+// (added to what is there), like those of the other layers; a standalone
+// parameter gets its gradient from autograd.
+struct GroupNorm : torch::autograd::Function<GroupNorm> {
+  static Variable forward(AutogradContext* ctx, const Variable& x,
+                          const Variable& gamma, const Variable& beta,
+                          const c10::optional<Variable>& residual, long groups,
+                          double eps, long act) {
+    auto out = group_norm_fwd(x, gamma, beta, groups, eps, act, residual);
+    // without an activation the gradient does not need the residual
+    ctx->save_for_backward({x, gamma, beta, out[1],
+                            act && residual ? *residual : torch::Tensor()});
+    ctx->saved_data["residual"] = residual.has_value();
+    ctx->saved_data["groups"] = (int64_t)groups;
+    ctx->saved_data["act"] = (int64_t)act;
+    if (gamma.requires_grad() && beta.requires_grad() &&
+        gamma.grad().defined() && beta.grad().defined()) {
+      ctx->saved_data["dgamma"] = gamma.grad();
+      ctx->saved_data["dbeta"] = beta.grad();
+    }
+    return out[0];
+  }
+
+  static variable_list backward(AutogradContext* ctx, variable_list grads) {
+    const auto saved = ctx->get_saved_variables();
+    const long groups = ctx->saved_data["groups"].toInt();
+    const long act = ctx->saved_data["act"].toInt();
+    const bool want_x = ctx->needs_input_grad(0);
+    const bool want_g = ctx->needs_input_grad(1);
+    const bool want_b = ctx->needs_input_grad(2);
+    const bool want_r = ctx->saved_data["residual"].toBool() &&
+                        ctx->needs_input_grad(3);
+    const auto view = ctx->saved_data.find("dgamma");
+    const bool direct = want_g && want_b && view != ctx->saved_data.end();
+    c10::optional<torch::Tensor> dgamma, dbeta;
+    if (direct) {
+      dgamma = view->second.toTensor();
+      dbeta = ctx->saved_data["dbeta"].toTensor();
+    }
+    const bool again = at::GradMode::is_enabled();
+    torch::Tensor dy;
+    std::vector<torch::Tensor> d;
+    {
+      at::NoGradGuard no_grad;
+      dy = grads[0].contiguous();
+      d = group_norm_bwd(dy, saved[0], saved[3], saved[1], saved[2], groups,
+                         act, if_defined(saved[4]), want_x, want_r && act,
+                         dgamma, dbeta);
+    }
+    if (want_r && !act) d[1] = dy;
+    variable_list out(7);
+    if (want_x) out[0] = d[0];
+    if (want_g && !direct) out[1] = d[2];
+    if (want_b && !direct) out[2] = d[3];
+    if (want_r) out[3] = d[1];
+    if (again)
+      for (auto& t : out)
+        if (t.defined()) t = once(t);
+    return out;
+  }
+};
+
+}  // namespace
+
+torch::Tensor group_norm(torch::Tensor x, torch::Tensor gamma,
+                         torch::Tensor beta,
+                         c10::optional<torch::Tensor> residual, long groups,
+                         double eps, long act) {
+  const torch::Tensor res = residual ? *residual : torch::Tensor();
+  const bool wanted =
+      at::GradMode::is_enabled() &&
+      (x.requires_grad() || gamma.requires_grad() || beta.requires_grad() ||
+       (res.defined() && res.requires_grad()));
+  if (!wanted) return group_norm_only(x, gamma, beta, groups, eps, act, residual);
+  if (c10::hip::currentStreamCaptureStatusMayInitCtx() !=
+      c10::hip::CaptureStatus::None) {
+    auto refuse = [](const torch::Tensor& t, bool param) {
+      TORCH_CHECK(!(t.defined() && t.requires_grad() && t.is_leaf() &&
+                    !(param && t.grad().defined())),
+                  "group_norm: a captured backward pass cannot accumulate "
+                  "into this leaf; give gamma and beta pre-allocated "
+                  "gradients, and make x and the residual in the captured "
+                  "region");
+    };
+    refuse(x, false);
+    refuse(gamma, true);
+    refuse(beta, true);
+    refuse(res, false);
+  }
+  return GroupNorm::apply(x, gamma, beta, residual, groups, eps, act);
+}
+
+}  // namespace eg

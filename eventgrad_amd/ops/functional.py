@@ -250,42 +250,6 @@ def batch_norm(x, gamma, beta, running_mean, running_var, training,
 _ACTIVATIONS = {"none": 0, "relu": 1, "silu": 2}
 
 
-class _GroupNormNHWC(torch.autograd.Function):
-    """Gradients of gamma and beta go straight into pre-allocated .grad views
-    (added to what is there), like those of the other layers; a standalone
-    parameter gets its gradient from autograd."""
-
-    @staticmethod
-    def forward(ctx, x, gamma, beta, residual, groups, eps, act):
-        y, stats = native().group_norm_fwd(x, gamma.detach(), beta.detach(),
-                                           groups, eps, act, residual)
-        # without an activation the gradient does not need the residual
-        ctx.save_for_backward(x, gamma, beta, stats,
-                              residual if act else None)
-        ctx.groups, ctx.act = groups, act
-        ctx.ggrad = gamma.grad if gamma.requires_grad else None
-        ctx.bgrad = beta.grad if beta.requires_grad else None
-        return y
-
-    @staticmethod
-    @torch.autograd.function.once_differentiable
-    def backward(ctx, dy):
-        x, gamma, beta, stats, residual = ctx.saved_tensors
-        want_x, want_g, want_b, want_r = ctx.needs_input_grad[:4]
-        dy = dy.contiguous()
-        direct = (want_g and want_b and ctx.ggrad is not None
-                  and ctx.bgrad is not None)
-        dx, dres, dgamma, dbeta = native().group_norm_bwd(
-            dy, x, stats, gamma.detach(), beta.detach(), ctx.groups, ctx.act,
-            residual, want_x, want_r and ctx.act != 0,
-            ctx.ggrad if direct else None, ctx.bgrad if direct else None)
-        if want_r and ctx.act == 0:
-            dres = dy
-        return (dx, dgamma if want_g and not direct else None,
-                dbeta if want_b and not direct else None, dres,
-                None, None, None)
-
-
 def _group_norm_plain(x, gamma, beta, groups, eps, act, residual):
     n, c = x.shape[:2]
     if x.numel() == 0:
@@ -336,22 +300,7 @@ def group_norm(x, gamma, beta, groups, eps=1e-5, activation="none",
                          f"{tuple(x.shape)}, got {tuple(residual.shape)}")
     if not native_path:
         return _group_norm_plain(x, gamma, beta, groups, eps, act, residual)
-    inputs = (x, gamma, beta) + (() if residual is None else (residual,))
-    if not (torch.is_grad_enabled() and any(t.requires_grad for t in inputs)):
-        return native().group_norm_fwd(x, gamma, beta, groups, eps, act,
-                                       residual)[0]
-    if torch.cuda.is_current_stream_capturing():
-        for t in inputs:
-            param = t is gamma or t is beta
-            if t.requires_grad and t.is_leaf and not (
-                    param and t.grad is not None):
-                raise RuntimeError(
-                    "group_norm: a captured backward pass cannot accumulate "
-                    "into this leaf; give gamma and beta pre-allocated "
-                    "gradients, and make x and the residual in the captured "
-                    "region")
-    return _GroupNormNHWC.apply(x, gamma, beta, residual, groups, float(eps),
-                                act)
+    return native().group_norm(x, gamma, beta, residual, groups, eps, act)
 
 
 # --------------------------------------------------------------------------

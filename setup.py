@@ -22,6 +22,8 @@ SRC = [
     "csrc/conv.hip",
     "csrc/bn.hip",
     "csrc/groupnorm.hip",
+    "csrc/groupnorm_bwd.hip",
+    "csrc/groupnorm_autograd.cpp",
     "csrc/adamw.hip",
     "csrc/pool.hip",
     "csrc/loss.hip",
