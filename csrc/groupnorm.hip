@@ -43,34 +43,37 @@ __global__ void __launch_bounds__(BLOCK) stats_kernel(
 }
 
 // One block a group: joins the channels and chunks of each,
-//   M2 = sum M2_i + count_i (mean_i - mean)^2.
+//   M2 = sum (M2_i + count_i mean_i^2) - M mean^2,
+// which in 64 bits leaves 16 digits less those of (mean / spread)^2.
 // Mean and rstd are kept in 64 bits: the sign of z decides a ReLU's gradient,
 // and where z is next to zero it is computed again from them.
-__global__ void __launch_bounds__(BLOCK) join_kernel(
+__global__ void __launch_bounds__(JOIN) join_kernel(
     const float2* __restrict__ part, double2* __restrict__ stats, long groups,
     int per_sample, int cpg, Deal d, double eps) {
-  __shared__ double slot[BLOCK / 64];
-  const long entries = (long)d.chunks * cpg;
+  __shared__ double slot[JOIN / 64];
+  const int entries = d.chunks * cpg;
+  const int down = JOIN / cpg, right = JOIN % cpg;
   const double m = (double)d.hw * cpg;
   for (long g = blockIdx.x; g < groups; g += gridDim.x) {
     const float2* p = part + g / per_sample * d.chunks * d.c +
                       g % per_sample * cpg;
-    double s = 0;
-    for (long i = threadIdx.x; i < entries; i += BLOCK) {
-      const int chunk = (int)(i / cpg);
-      const int rows = min(d.per_chunk, d.hw - chunk * d.per_chunk);
-      s += (double)rows * p[(long)chunk * d.c + i % cpg].x;
+    double s = 0, q = 0;
+    int chunk = threadIdx.x / cpg, ch = threadIdx.x % cpg;
+#pragma unroll 4
+    for (int i = threadIdx.x; i < entries; i += JOIN) {
+      const float2 e = p[(long)chunk * d.c + ch];
+      const double rows = min(d.per_chunk, d.hw - chunk * d.per_chunk);
+      s += rows * e.x;
+      q += (double)e.y + rows * e.x * e.x;
+      chunk += down;
+      ch += right;
+      if (ch >= cpg) {
+        ch -= cpg;
+        ++chunk;
+      }
     }
     const double mean = add_block(s, slot) / m;
-    double q = 0;
-    for (long i = threadIdx.x; i < entries; i += BLOCK) {
-      const int chunk = (int)(i / cpg);
-      const int rows = min(d.per_chunk, d.hw - chunk * d.per_chunk);
-      const float2 e = p[(long)chunk * d.c + i % cpg];
-      const double off = (double)e.x - mean;
-      q += (double)e.y + (double)rows * off * off;
-    }
-    const double var = add_block(q, slot) / m;
+    const double var = add_block(q, slot) / m - mean * mean;
     if (threadIdx.x == 0) {
       // a variance cannot be below zero, and NaN stays NaN
       stats[g] = make_double2(mean, 1.0 / sqrt((var < 0 ? 0 : var) + eps));
@@ -78,48 +81,56 @@ __global__ void __launch_bounds__(BLOCK) join_kernel(
   }
 }
 
-template <typename T, int V>
+template <typename T, int V, int ACT>
 __global__ void __launch_bounds__(BLOCK) apply_kernel(
     const T* __restrict__ x, const T* __restrict__ res, T* __restrict__ y,
-    const double2* __restrict__ stats, const float* __restrict__ gamma,
-    const float* __restrict__ beta, int groups, int cpg, int act, Deal d) {
+    unsigned char* __restrict__ mask, const double2* __restrict__ stats,
+    const float* __restrict__ gamma, const float* __restrict__ beta,
+    int groups, int cpg, Deal d) {
   const Place at(d);
   if (!at.on) return;
-  float mean[V], scale[V], shift[V];
+  const int c0 = at.col * V;
+  const double2* sample = stats + (long)at.n * groups;
+  float mean[V], scale[V], shift[V], limit = 0.f;
 #pragma unroll
   for (int j = 0; j < V; ++j) {
-    const int ch = at.col * V + j;
-    const double2 st = stats[(long)at.n * groups + ch / cpg];
+    const double2 st = sample[(c0 + j) / cpg];
     mean[j] = (float)st.x;
-    scale[j] = (float)(gamma[ch] * st.y);
-    shift[j] = beta[ch];
+    scale[j] = (float)(gamma[c0 + j] * st.y);
+    shift[j] = beta[c0 + j];
+    limit = fmaxf(limit, fabsf(scale[j] * mean[j]) + 2.f * fabsf(shift[j]));
   }
-  const long base = ((long)at.n * d.hw + at.begin) * d.c + at.col * V;
+  limit *= 0x1p-20f;
+  const long base = ((long)at.n * d.hw + at.begin) * d.c + c0;
 #pragma unroll 2
   for (int k = at.r; k < at.count; k += d.rows) {
     const long i = base + (long)k * d.c;
     Vec<T, V> a = load<T, V>(x + i), b;
     if (res) b = load<T, V>(res + i);
-#pragma unroll
-    for (int j = 0; j < V; ++j) {
-      float z = fmaf((float)a.v[j] - mean[j], scale[j], shift[j]);
-      if (res) z += (float)b.v[j];
-      a.v[j] = (T)activate(z, act);
-    }
+    auto exact = [&](int j) {
+      const double2 st = sample[(c0 + j) / cpg];
+      const double z = ((double)(float)x[i + j] - st.x) * st.y *
+                           (double)gamma[c0 + j] + (double)beta[c0 + j];
+      return res ? z + (double)(float)res[i + j] : z;
+    };
+    const unsigned bits = activate<T, V, V, ACT>(a, b, res, mean, scale,
+                                                 shift, limit, exact);
     store<T, V>(y + i, a);
+    if (ACT == RELU_BITS) mask[i / V] = (unsigned char)bits;
   }
 }
 
 // The slab in one pass. P: statistics that a thread needs, 1 where a vector
 // lies within a group, else one a channel.
-template <typename T, int V, int I, int P>
+template <typename T, int V, int I, int P, int ACT>
 __global__ void __launch_bounds__(SLAB) slab_kernel(
     const T* __restrict__ x, const T* __restrict__ res, T* __restrict__ y,
-    double2* __restrict__ stats, const float* __restrict__ gamma,
-    const float* __restrict__ beta, double eps, int act, Slab d) {
+    unsigned char* __restrict__ mask, double2* __restrict__ stats,
+    const float* __restrict__ gamma, const float* __restrict__ beta,
+    double eps, Slab d) {
   __shared__ float table[SLAB * P];
   __shared__ double mean_of[SLAB];
-  __shared__ float rstd_of[SLAB];
+  __shared__ double rstd_of[SLAB];
   const Spot at(d, V);
   const int w = P == 1 ? d.cpg / V : d.cpg;
   const double m = (double)d.hw * d.cpg;
@@ -166,20 +177,23 @@ __global__ void __launch_bounds__(SLAB) slab_kernel(
   __syncthreads();
   add_groups<double>(table, d.rows, w, d, [&](int q, double t) {
     const double rstd = 1.0 / sqrt(t / m + eps);
-    rstd_of[q] = (float)rstd;
+    rstd_of[q] = rstd;
     if (stats)
       stats[(long)at.n * d.groups + at.first / d.cpg + q] =
           make_double2(mean_of[q], rstd);
   });
   __syncthreads();
   if (!at.on) return;
-  float scale[V], shift[V];
+  const int c0 = at.first + at.lane * V;
+  float scale[V], shift[V], limit = 0.f;
 #pragma unroll
   for (int j = 0; j < V; ++j) {
-    const int ch = at.first + at.lane * V + j;
-    scale[j] = gamma[ch] * rstd_of[(at.lane * V + (P == 1 ? 0 : j)) / d.cpg];
-    shift[j] = beta[ch];
+    const int p = P == 1 ? 0 : j;
+    scale[j] = (float)(gamma[c0 + j] * rstd_of[(at.lane * V + p) / d.cpg]);
+    shift[j] = beta[c0 + j];
+    limit = fmaxf(limit, fabsf(scale[j] * mean[p]) + 2.f * fabsf(shift[j]));
   }
+  limit *= 0x1p-20f;
 #pragma unroll
   for (int k = 0; k < I; ++k) {
     const int row = at.r + k * d.rows;
@@ -187,26 +201,28 @@ __global__ void __launch_bounds__(SLAB) slab_kernel(
     const long i = base + (long)row * d.c;
     Vec<T, V> b;
     if (res) b = load<T, V>(res + i);
-#pragma unroll
-    for (int j = 0; j < V; ++j) {
-      float z = fmaf((float)a[k].v[j] - mean[P == 1 ? 0 : j], scale[j],
-                     shift[j]);
-      if (res) z += (float)b.v[j];
-      a[k].v[j] = (T)activate(z, act);
-    }
+    auto exact = [&](int j) {
+      const int q = (at.lane * V + j) / d.cpg;
+      const double z = ((double)(float)x[i + j] - mean_of[q]) * rstd_of[q] *
+                           (double)gamma[c0 + j] + (double)beta[c0 + j];
+      return res ? z + (double)(float)res[i + j] : z;
+    };
+    const unsigned bits = activate<T, V, P, ACT>(a[k], b, res, mean, scale,
+                                                 shift, limit, exact);
     store<T, V>(y + i, a[k]);
+    if (ACT == RELU_BITS) mask[i / V] = (unsigned char)bits;
   }
 }
 
 }  // namespace gn
 
-// y, and into stats per sample and group (mean, rstd) in 64 bits; stats is
-// undefined where nobody wants them
+// y; and where `stats` is given per sample and group (mean, rstd) in 64 bits,
+// and for a ReLU the bits of z > 0
 static torch::Tensor forward(const torch::Tensor& x,
                              const torch::Tensor& gamma,
                              const torch::Tensor& beta, const gn::Shape& s,
                              double eps, long act, const torch::Tensor& res,
-                             torch::Tensor* stats) {
+                             torch::Tensor* stats, torch::Tensor* mask) {
   using namespace gn;
   TORCH_CHECK(eps >= 0, "group_norm: eps must not be negative");
   const c10::DeviceGuard guard(x.device());
@@ -219,6 +235,11 @@ static torch::Tensor forward(const torch::Tensor& x,
   const int v = width(s, size, {x.data_ptr(), y.data_ptr(), r});
   const float* gm = gamma.data_ptr<float>();
   const float* bt = beta.data_ptr<float>();
+  unsigned char* mk = nullptr;
+  if (mask && act == RELU) {
+    *mask = torch::empty({x.numel() / v}, x.options().dtype(torch::kUInt8));
+    mk = mask->data_ptr<unsigned char>();
+  }
   const hipStream_t stream = cur_stream();
   const Cut slab = cut(s, v, size, FWD_VECTORS);
   if (slab.threads) {
@@ -227,12 +248,14 @@ static torch::Tensor forward(const torch::Tensor& x,
       using G = decltype(tag);
       using T = typename G::type;
       if constexpr (G::i <= FWD_VECTORS) {
-        slab_kernel<T, G::v, G::i, G::p>
-            <<<(unsigned)(s.n * slab.d.slices), slab.threads, 0, stream>>>(
-                reinterpret_cast<const T*>(x.data_ptr()),
-                reinterpret_cast<const T*>(r),
-                reinterpret_cast<T*>(y.data_ptr()), st, gm, bt, eps, (int)act,
-                slab.d);
+        with_act(act, mk, [&](auto a) {
+          slab_kernel<T, G::v, G::i, G::p, decltype(a)::v>
+              <<<(unsigned)(s.n * slab.d.slices), slab.threads, 0, stream>>>(
+                  reinterpret_cast<const T*>(x.data_ptr()),
+                  reinterpret_cast<const T*>(r),
+                  reinterpret_cast<T*>(y.data_ptr()), mk, st, gm, bt, eps,
+                  slab.d);
+        });
       }
     });
     return y;
@@ -252,26 +275,29 @@ static torch::Tensor forward(const torch::Tensor& x,
     constexpr int V = decltype(tag)::v;
     const T* xp = reinterpret_cast<const T*>(x.data_ptr());
     stats_kernel<T, V><<<grid, BLOCK, 0, stream>>>(xp, pt, d);
-    join_kernel<<<joins, BLOCK, 0, stream>>>(pt, st, all, s.groups, s.cpg, d,
+    join_kernel<<<joins, JOIN, 0, stream>>>(pt, st, all, s.groups, s.cpg, d,
                                              eps);
-    apply_kernel<T, V><<<grid, BLOCK, 0, stream>>>(
-        xp, reinterpret_cast<const T*>(r), reinterpret_cast<T*>(y.data_ptr()),
-        st, gm, bt, s.groups, s.cpg, (int)act, d);
+    with_act(act, mk, [&](auto a) {
+      apply_kernel<T, V, decltype(a)::v><<<grid, BLOCK, 0, stream>>>(
+          xp, reinterpret_cast<const T*>(r),
+          reinterpret_cast<T*>(y.data_ptr()), mk, st, gm, bt, s.groups, s.cpg,
+          d);
+    });
   });
   return y;
 }
 
-// y and the statistics that group_norm_bwd takes
+// y, and the statistics and bits that group_norm_bwd takes
 std::vector<torch::Tensor> group_norm_fwd(torch::Tensor x,
                                           torch::Tensor gamma,
                                           torch::Tensor beta, long groups,
                                           double eps, long act,
                                           c10::optional<torch::Tensor> res) {
   const auto s = gn::shape_of(x, gamma, beta, groups, act, res);
-  torch::Tensor stats;
+  torch::Tensor stats, mask;
   auto y = forward(x, gamma, beta, s, eps, act,
-                   res ? *res : torch::Tensor(), &stats);
-  return {y, stats};
+                   res ? *res : torch::Tensor(), &stats, &mask);
+  return {y, stats, mask};
 }
 
 // y alone
@@ -280,7 +306,7 @@ torch::Tensor group_norm_only(torch::Tensor x, torch::Tensor gamma,
                               long act, c10::optional<torch::Tensor> res) {
   const auto s = gn::shape_of(x, gamma, beta, groups, act, res);
   return forward(x, gamma, beta, s, eps, act, res ? *res : torch::Tensor(),
-                 nullptr);
+                 nullptr, nullptr);
 }
 
 }  // namespace eg

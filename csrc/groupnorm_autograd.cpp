@@ -18,8 +18,8 @@ torch::Tensor group_norm_only(torch::Tensor, torch::Tensor, torch::Tensor,
                               c10::optional<torch::Tensor>);
 std::vector<torch::Tensor> group_norm_bwd(
     torch::Tensor, torch::Tensor, torch::Tensor, torch::Tensor, torch::Tensor,
-    long, long, c10::optional<torch::Tensor>, bool, bool,
-    c10::optional<torch::Tensor>, c10::optional<torch::Tensor>);
+    long, long, c10::optional<torch::Tensor>, c10::optional<torch::Tensor>,
+    bool, bool, c10::optional<torch::Tensor>, c10::optional<torch::Tensor>);
 
 namespace {
 
@@ -49,9 +49,11 @@ struct GroupNorm : torch::autograd::Function<GroupNorm> {
                           const c10::optional<Variable>& residual, long groups,
                           double eps, long act) {
     auto out = group_norm_fwd(x, gamma, beta, groups, eps, act, residual);
-    // without an activation the gradient does not need the residual
+    // a ReLU's gradient needs the bits that the pass left (out[2]) in the
+    // residual's place, and without an activation it needs neither
     ctx->save_for_backward({x, gamma, beta, out[1],
-                            act && residual ? *residual : torch::Tensor()});
+                            act == 2 && residual ? *residual : torch::Tensor(),
+                            out[2]});
     ctx->saved_data["residual"] = residual.has_value();
     ctx->saved_data["groups"] = (int64_t)groups;
     ctx->saved_data["act"] = (int64_t)act;
@@ -86,8 +88,8 @@ struct GroupNorm : torch::autograd::Function<GroupNorm> {
       at::NoGradGuard no_grad;
       dy = grads[0].contiguous();
       d = group_norm_bwd(dy, saved[0], saved[3], saved[1], saved[2], groups,
-                         act, if_defined(saved[4]), want_x, want_r && act,
-                         dgamma, dbeta);
+                         act, if_defined(saved[4]), if_defined(saved[5]),
+                         want_x, want_r && act, dgamma, dbeta);
     }
     if (want_r && !act) d[1] = dy;
     variable_list out(7);

@@ -5,77 +5,61 @@ namespace gn {
 
 // ---- backward -------------------------------------------------------------
 
-// What a thread keeps of its V channels, and dz from them.
-template <typename T, int V>
+// What a thread keeps of its V channels. SILU: dz is dy times the slope at z;
+// without, it is dy where the forward pass left a bit, or everywhere.
+template <typename T, int V, bool SILU_>
 struct Channels {
-  float mean[V], rstd[V], gamma[V], beta[V];
-  const double2* stats;
-  int cpg, first;
+  float mean[V], rstd[V], gamma[V], beta[SILU_ ? V : 1];
 
   __device__ __forceinline__ Channels(const double2* sample, int c0,
-                                      const float* g, const float* b, int n) {
-    stats = sample;
-    cpg = n;
-    first = c0;
+                                      const float* g, const float* b,
+                                      int cpg) {
 #pragma unroll
     for (int j = 0; j < V; ++j) {
-      const double2 st = sample[(c0 + j) / n];
+      const double2 st = sample[(c0 + j) / cpg];
       mean[j] = (float)st.x;
       rstd[j] = (float)st.y;
       gamma[j] = g[c0 + j];
-      beta[j] = b[c0 + j];
+      if (SILU_) beta[j] = b[c0 + j];
     }
   }
 
-  // xh, and dz = dy act'(z). z is off by a few 2^-24 of the terms that make
-  // it; where that could turn its sign it is taken again in 64 bits.
-  __device__ __forceinline__ float dz(int j, float x, float r, float dy,
-                                      int act, float& xh) const {
-    xh = (x - mean[j]) * rstd[j];
-    if (act == NONE) return dy;
-    float z = fmaf(xh, gamma[j], beta[j]) + r;
-    if (act == SILU) {
-      const float s = sigmoid(z);
-      return dy * (s * fmaf(z, 1.f - s, 1.f));
-    }
-    const float unsure =
-        0x1p-20f * (fabsf(gamma[j] * rstd[j] * mean[j]) +
-                    2.f * (fabsf(beta[j]) + fabsf(r)));
-    if (fabsf(z) <= unsure) {
-      const double2 st = stats[(first + j) / cpg];
-      const double e = ((double)x - st.x) * st.y * (double)gamma[j] +
-                       (double)beta[j] + (double)r;
-      return e <= 0.0 ? 0.f : dy;
-    }
-    return z <= 0.f ? 0.f : dy;
+  __device__ __forceinline__ float dz(int j, float xh, float r,
+                                      float dy) const {
+    if (!SILU_) return dy;
+    const float z = fmaf(xh, gamma[j], beta[j]) + r;
+    const float s = sigmoid(z);
+    return dy * (s * fmaf(z, 1.f - s, 1.f));
   }
 };
 
 // Each channel's sums of dz and of dz xh over one chunk of rows.
-template <typename T, int V>
+template <typename T, int V, bool SILU_>
 __global__ void __launch_bounds__(BLOCK) bwd_sums_kernel(
     const T* __restrict__ dy, const T* __restrict__ x,
-    const T* __restrict__ res, const double2* __restrict__ stats,
-    const float* __restrict__ gamma, const float* __restrict__ beta,
-    float2* __restrict__ part, int groups, int cpg, int act, Deal d) {
+    const T* __restrict__ res, const unsigned char* __restrict__ mask,
+    const double2* __restrict__ stats, const float* __restrict__ gamma,
+    const float* __restrict__ beta, float2* __restrict__ part, int groups,
+    int cpg, Deal d) {
   __shared__ float slot[BLOCK / 2 * 2 * V];
   const Place at(d);
   float sums[2 * V] = {};
   if (at.on) {
-    const Channels<T, V> ch(stats + (long)at.n * groups, at.col * V, gamma,
-                            beta, cpg);
+    const Channels<T, V, SILU_> ch(stats + (long)at.n * groups, at.col * V,
+                                   gamma, beta, cpg);
     const long base = ((long)at.n * d.hw + at.begin) * d.c + at.col * V;
 #pragma unroll 2
     for (int k = at.r; k < at.count; k += d.rows) {
       const long i = base + (long)k * d.c;
-      const Vec<T, V> a = load<T, V>(x + i), g = load<T, V>(dy + i);
-      Vec<T, V> b;
-      if (res) b = load<T, V>(res + i);
+      const Vec<T, V> a = load<T, V>(x + i);
+      Vec<T, V> g = load<T, V>(dy + i), b;
+      if (SILU_ && res) b = load<T, V>(res + i);
+      if (!SILU_ && mask) keep<T, V>(g, mask[i / V]);
 #pragma unroll
       for (int j = 0; j < V; ++j) {
-        float xh;
-        const float dz = ch.dz(j, (float)a.v[j], res ? (float)b.v[j] : 0.f,
-                               (float)g.v[j], act, xh);
+        const float xh = ((float)a.v[j] - ch.mean[j]) * ch.rstd[j];
+        const float dz = ch.dz(j, xh, SILU_ && res ? (float)b.v[j] : 0.f,
+                               (float)g.v[j]);
         sums[j] += dz;
         sums[V + j] = fmaf(dz, xh, sums[V + j]);
       }
@@ -91,15 +75,15 @@ __global__ void __launch_bounds__(BLOCK) bwd_sums_kernel(
 
 // One block a group: each channel's sums over the chunks, for dgamma and
 // dbeta, and the group's s1 and s2.
-__global__ void __launch_bounds__(BLOCK) bwd_join_kernel(
+__global__ void __launch_bounds__(JOIN) bwd_join_kernel(
     const float2* __restrict__ part, const float* __restrict__ gamma,
     float2* __restrict__ channel, float2* __restrict__ group, long groups,
     int per_sample, int cpg, int across, Deal d) {
   // across: threads side by side over channels, a power of two
-  __shared__ float2 slot[BLOCK];
-  __shared__ float sums[BLOCK / 64];
+  __shared__ float2 slot[JOIN];
+  __shared__ float sums[JOIN / 64];
   const int lane = threadIdx.x % across, share = threadIdx.x / across;
-  const int shares = BLOCK / across;
+  const int shares = JOIN / across;
   const float inv = 1.f / ((float)d.hw * (float)cpg);
   for (long g = blockIdx.x; g < groups; g += gridDim.x) {
     const long n = g / per_sample;
@@ -139,48 +123,47 @@ __global__ void __launch_bounds__(BLOCK) bwd_join_kernel(
 }
 
 // dgamma and dbeta: each channel's sums over the samples, added to what is
-// there (a gradient's view in the flat space) or put down.
-constexpr int PC = 32, PN = 32;
+// there (a gradient's view in the flat space) or put down. 16 channels, a
+// cache line of pairs, by 64 shares of the samples.
+constexpr int PC = 16, PN = 64;
 __global__ void __launch_bounds__(PC* PN) bwd_params_kernel(
     const float2* __restrict__ channel, float* __restrict__ dgamma,
     float* __restrict__ dbeta, long n, int c, int add) {
-  __shared__ float2 slot[PN / 2][PC];
+  __shared__ Pair slot[PC * PN / 64][PC];
   const int lane = threadIdx.x % PC, share = threadIdx.x / PC;
   const int ch = blockIdx.x * PC + lane;
-  float2 s = make_float2(0.f, 0.f);
+  Pair s = {0.f, 0.f};
   if (ch < c) {
+#pragma unroll 4
     for (long k = share; k < n; k += PN) {
       const float2 e = channel[k * c + ch];
-      s.x += e.x;
-      s.y += e.y;
+      s += Pair{e.x, e.y};
     }
   }
-  for (int half = PN / 2; half; half /= 2) {
-    if (share >= half && share < 2 * half) slot[share - half][lane] = s;
-    __syncthreads();
-    if (share < half) {
-      s.x += slot[share][lane].x;
-      s.y += slot[share][lane].y;
-    }
-    __syncthreads();
-  }
-  if (share == 0 && ch < c) {
-    dgamma[ch] = add ? dgamma[ch] + s.y : s.y;
-    dbeta[ch] = add ? dbeta[ch] + s.x : s.x;
+  s += across(s, 16);
+  s += across(s, 32);
+  if (threadIdx.x % 64 < PC) slot[threadIdx.x / 64][lane] = s;
+  __syncthreads();
+  if (threadIdx.x < PC && ch < c) {
+    Pair t = {0.f, 0.f};
+#pragma unroll
+    for (int w = 0; w < PC * PN / 64; ++w) t += slot[w][lane];
+    dgamma[ch] = add ? dgamma[ch] + t.b : t.b;
+    dbeta[ch] = add ? dbeta[ch] + t.a : t.a;
   }
 }
 
-template <typename T, int V>
+template <typename T, int V, bool SILU_>
 __global__ void __launch_bounds__(BLOCK) bwd_apply_kernel(
     const T* __restrict__ dy, const T* __restrict__ x,
-    const T* __restrict__ res, const double2* __restrict__ stats,
-    const float* __restrict__ gamma, const float* __restrict__ beta,
-    const float2* __restrict__ group, T* __restrict__ dx,
-    T* __restrict__ dres, int groups, int cpg, int act, Deal d) {
+    const T* __restrict__ res, const unsigned char* __restrict__ mask,
+    const double2* __restrict__ stats, const float* __restrict__ gamma,
+    const float* __restrict__ beta, const float2* __restrict__ group,
+    T* __restrict__ dx, T* __restrict__ dres, int groups, int cpg, Deal d) {
   const Place at(d);
   if (!at.on) return;
-  const Channels<T, V> ch(stats + (long)at.n * groups, at.col * V, gamma,
-                          beta, cpg);
+  const Channels<T, V, SILU_> ch(stats + (long)at.n * groups, at.col * V,
+                                 gamma, beta, cpg);
   float s1[V], s2[V];
 #pragma unroll
   for (int j = 0; j < V; ++j) {
@@ -192,47 +175,69 @@ __global__ void __launch_bounds__(BLOCK) bwd_apply_kernel(
 #pragma unroll 2
   for (int k = at.r; k < at.count; k += d.rows) {
     const long i = base + (long)k * d.c;
-    const Vec<T, V> a = load<T, V>(x + i), g = load<T, V>(dy + i);
-    Vec<T, V> b, u;
-    if (res) b = load<T, V>(res + i);
+    const Vec<T, V> a = load<T, V>(x + i);
+    Vec<T, V> g = load<T, V>(dy + i), b, u;
+    if (SILU_ && res) b = load<T, V>(res + i);
+    if (!SILU_ && mask) keep<T, V>(g, mask[i / V]);
 #pragma unroll
     for (int j = 0; j < V; ++j) {
-      float xh;
-      const float dz = ch.dz(j, (float)a.v[j], res ? (float)b.v[j] : 0.f,
-                             (float)g.v[j], act, xh);
+      const float xh = ((float)a.v[j] - ch.mean[j]) * ch.rstd[j];
+      const float dz = ch.dz(j, xh, SILU_ && res ? (float)b.v[j] : 0.f,
+                             (float)g.v[j]);
       u.v[j] = (T)(ch.rstd[j] *
                    (fmaf(dz, ch.gamma[j], -s1[j]) - xh * s2[j]));
-      b.v[j] = (T)dz;
+      if (SILU_) g.v[j] = (T)dz;
     }
     if (dx) store<T, V>(dx + i, u);
-    if (dres) store<T, V>(dres + i, b);
+    if (dres) store<T, V>(dres + i, g);
   }
 }
 
 // The slab in one pass: x and dy stay in registers between the sums and dx.
-template <typename T, int V, int I, int P>
+template <typename T, int V, int I, int P, bool SILU_>
 __global__ void __launch_bounds__(SLAB) bwd_slab_kernel(
     const T* __restrict__ dy, const T* __restrict__ x,
-    const T* __restrict__ res, const double2* __restrict__ stats,
-    const float* __restrict__ gamma, const float* __restrict__ beta,
-    float2* __restrict__ channel, T* __restrict__ dx, T* __restrict__ dres,
-    int act, Slab d) {
+    const T* __restrict__ res, const unsigned char* __restrict__ mask,
+    const double2* __restrict__ stats, const float* __restrict__ gamma,
+    const float* __restrict__ beta, float2* __restrict__ channel,
+    T* __restrict__ dx, T* __restrict__ dres, Slab d) {
   __shared__ Pair table[SLAB * V];
   __shared__ Pair group[SLAB];
   const Spot at(d, V);
   const long base = (long)at.n * d.hw * d.c + at.first + at.lane * V;
   Vec<T, V> a[I], g[I];
+  unsigned bits[I];
 #pragma unroll
   for (int k = 0; k < I; ++k) {
     const int row = at.r + k * d.rows;
     if (at.on && row < d.hw) {
-      a[k] = load<T, V>(x + base + (long)row * d.c);
-      g[k] = load<T, V>(dy + base + (long)row * d.c);
+      const long i = base + (long)row * d.c;
+      a[k] = load<T, V>(x + i);
+      g[k] = load<T, V>(dy + i);
+      if (!SILU_ && mask) bits[k] = mask[i / V];
     }
   }
-  const Channels<T, V> ch(stats + (long)at.n * d.groups,
-                          at.on ? at.first + at.lane * V : 0, gamma, beta,
-                          d.cpg);
+  // mean, rstd, s1 and s2 of a thread's channels: one, or P
+  const double2* sample = stats + (long)at.n * d.groups;
+  const int c0 = at.on ? at.first + at.lane * V : 0;
+  float mean[P], rstd[P], gam[V], bet[SILU_ ? V : 1];
+#pragma unroll
+  for (int j = 0; j < P; ++j) {
+    const double2 st = sample[(c0 + j) / d.cpg];
+    mean[j] = (float)st.x;
+    rstd[j] = (float)st.y;
+  }
+#pragma unroll
+  for (int j = 0; j < V; ++j) {
+    gam[j] = gamma[c0 + j];
+    if (SILU_) bet[j] = beta[c0 + j];
+  }
+  auto slope = [&](int j, float off, float r) {
+    const float z = fmaf(off * rstd[P == 1 ? 0 : j], gam[j], bet[j]) + r;
+    const float s = sigmoid(z);
+    return s * fmaf(z, 1.f - s, 1.f);
+  };
+  // sums of dz and of dz (x - mean); the latter's rstd comes at the end
   float s[2 * V] = {};
 #pragma unroll
   for (int k = 0; k < I; ++k) {
@@ -240,24 +245,26 @@ __global__ void __launch_bounds__(SLAB) bwd_slab_kernel(
     if (at.on && row < d.hw) {
       const long i = base + (long)row * d.c;
       Vec<T, V> b;
-      if (res) b = load<T, V>(res + i);
+      if (SILU_ && res) b = load<T, V>(res + i);
+      if (!SILU_ && mask) keep<T, V>(g[k], bits[k]);
 #pragma unroll
       for (int j = 0; j < V; ++j) {
-        float xh;
-        const float dz = ch.dz(j, (float)a[k].v[j], res ? (float)b.v[j] : 0.f,
-                               (float)g[k].v[j], act, xh);
+        const float off = (float)a[k].v[j] - mean[P == 1 ? 0 : j];
+        float dz = (float)g[k].v[j];
+        if (SILU_) {
+          dz *= slope(j, off, res ? (float)b.v[j] : 0.f);
+          b.v[j] = (T)dz;
+        }
         s[j] += dz;
-        s[V + j] = fmaf(dz, xh, s[V + j]);
-        b.v[j] = (T)dz;
-        // a ReLU's dz is dy or nothing: the register holds it exactly
-        if (act == RELU) g[k].v[j] = (T)dz;
+        s[V + j] = fmaf(dz, off, s[V + j]);
       }
-      if (dres) store<T, V>(dres + i, b);
+      if (dres) store<T, V>(dres + i, SILU_ ? b : g[k]);
     }
   }
 #pragma unroll
   for (int j = 0; j < V; ++j)
-    table[threadIdx.x * V + j] = Pair{s[j], s[V + j]};
+    table[threadIdx.x * V + j] =
+        Pair{s[j], s[V + j] * rstd[P == 1 ? 0 : j]};
   __syncthreads();
   // rows of a channel: first in `parts` shares, in place, then those
   const int width = d.lanes * V;
@@ -284,27 +291,28 @@ __global__ void __launch_bounds__(SLAB) bwd_slab_kernel(
   });
   __syncthreads();
   if (!dx || !at.on) return;
-  Pair t[P];
+  // dx = (rstd gamma) dz - (rstd^2 s2) (x - mean) - rstd s1
+  float by_x[P], less[P];
 #pragma unroll
-  for (int j = 0; j < P; ++j) t[j] = group[(at.lane * V + j) / d.cpg];
+  for (int j = 0; j < P; ++j) {
+    const Pair t = group[(at.lane * V + j) / d.cpg];
+    by_x[j] = -rstd[j] * rstd[j] * t.b;
+    less[j] = -rstd[j] * t.a;
+  }
 #pragma unroll
   for (int k = 0; k < I; ++k) {
     const int row = at.r + k * d.rows;
     if (row >= d.hw) break;
     const long i = base + (long)row * d.c;
     Vec<T, V> b;
-    if (res && act == SILU) b = load<T, V>(res + i);
+    if (SILU_ && res) b = load<T, V>(res + i);
 #pragma unroll
     for (int j = 0; j < V; ++j) {
       const int p = P == 1 ? 0 : j;
-      float xh, dz = (float)g[k].v[j];
-      if (act == SILU)
-        dz = ch.dz(j, (float)a[k].v[j], res ? (float)b.v[j] : 0.f, dz, act,
-                   xh);
-      else
-        xh = ((float)a[k].v[j] - ch.mean[j]) * ch.rstd[j];
-      a[k].v[j] =
-          (T)(ch.rstd[j] * (fmaf(dz, ch.gamma[j], -t[p].a) - xh * t[p].b));
+      const float off = (float)a[k].v[j] - mean[p];
+      float dz = (float)g[k].v[j];
+      if (SILU_) dz *= slope(j, off, res ? (float)b.v[j] : 0.f);
+      a[k].v[j] = (T)fmaf(dz, gam[j] * rstd[p], fmaf(off, by_x[p], less[p]));
     }
     store<T, V>(dx + i, a[k]);
   }
@@ -314,12 +322,12 @@ __global__ void __launch_bounds__(SLAB) bwd_slab_kernel(
 
 // dx, the residual's gradient, dgamma and dbeta; an undefined tensor where
 // one is not wanted. The parameters' gradients are added to dgamma_out and
-// dbeta_out where those are given.
+// dbeta_out where those are given. mask: a ReLU's bits, res: of a SiLU.
 std::vector<torch::Tensor> group_norm_bwd(
     torch::Tensor dy, torch::Tensor x, torch::Tensor stats,
     torch::Tensor gamma, torch::Tensor beta, long groups, long act,
-    c10::optional<torch::Tensor> res, bool want_dx, bool want_dres,
-    c10::optional<torch::Tensor> dgamma_out,
+    c10::optional<torch::Tensor> res, c10::optional<torch::Tensor> mask,
+    bool want_dx, bool want_dres, c10::optional<torch::Tensor> dgamma_out,
     c10::optional<torch::Tensor> dbeta_out) {
   using namespace gn;
   const Shape s = shape_of(x, gamma, beta, groups, act, res);
@@ -364,7 +372,22 @@ std::vector<torch::Tensor> group_norm_bwd(
   void* dxp = want_dx ? dx.data_ptr() : nullptr;
   void* drp = want_dres ? dres.data_ptr() : nullptr;
   const int size = (int)x.element_size();
-  const int v = width(s, size, {x.data_ptr(), dy.data_ptr(), r, dxp, drp});
+  // the bits are a byte for each vector of the forward pass
+  int v = width(s, size, {x.data_ptr(), dy.data_ptr(), r, dxp, drp});
+  const unsigned char* mk = nullptr;
+  if (act == RELU) {
+    TORCH_CHECK(mask && mask->device() == x.device() &&
+                    mask->scalar_type() == torch::kUInt8 &&
+                    mask->is_contiguous() && mask->numel() > 0 &&
+                    x.numel() % mask->numel() == 0,
+                "group_norm: mask must be that of the forward pass");
+    mk = mask->data_ptr<unsigned char>();
+    const int was = (int)(x.numel() / mask->numel());
+    if (v < was) dy = dy.clone();      // of lesser alignment than x
+    v = was;
+    TORCH_CHECK(v <= width(s, size, {x.data_ptr(), dy.data_ptr(), dxp, drp}),
+                "group_norm: mask must be that of the forward pass");
+  }
   const auto* st = reinterpret_cast<const double2*>(stats.data_ptr());
   const float* gm = gamma.data_ptr<float>();
   const float* bt = beta.data_ptr<float>();
@@ -382,13 +405,16 @@ std::vector<torch::Tensor> group_norm_bwd(
       using G = decltype(tag);
       using T = typename G::type;
       if constexpr (G::i <= BWD_VECTORS) {
-        bwd_slab_kernel<T, G::v, G::i, G::p>
-            <<<(unsigned)(s.n * slab.d.slices), slab.threads, 0, stream>>>(
-                reinterpret_cast<const T*>(dy.data_ptr()),
-                reinterpret_cast<const T*>(x.data_ptr()),
-                reinterpret_cast<const T*>(r), st, gm, bt, cp,
-                reinterpret_cast<T*>(dxp), reinterpret_cast<T*>(drp),
-                (int)act, slab.d);
+        const unsigned blocks = (unsigned)(s.n * slab.d.slices);
+        auto run = [&](auto kernel) {
+          kernel<<<blocks, slab.threads, 0, stream>>>(
+              reinterpret_cast<const T*>(dy.data_ptr()),
+              reinterpret_cast<const T*>(x.data_ptr()),
+              reinterpret_cast<const T*>(r), mk, st, gm, bt, cp,
+              reinterpret_cast<T*>(dxp), reinterpret_cast<T*>(drp), slab.d);
+        };
+        if (act == SILU) run(bwd_slab_kernel<T, G::v, G::i, G::p, true>);
+        else run(bwd_slab_kernel<T, G::v, G::i, G::p, false>);
       }
     });
     params();
@@ -404,22 +430,31 @@ std::vector<torch::Tensor> group_norm_bwd(
   auto* pt = reinterpret_cast<float2*>(part.data_ptr());
   auto* gp = reinterpret_cast<float2*>(group.data_ptr());
   int across = 1;
-  while (across < s.cpg && across < BLOCK) across *= 2;
+  while (across < s.cpg && across < JOIN) across *= 2;
   with_type(x.scalar_type(), v, [&](auto tag) {
     using T = typename decltype(tag)::type;
     constexpr int V = decltype(tag)::v;
     const T* xp = reinterpret_cast<const T*>(x.data_ptr());
     const T* yp = reinterpret_cast<const T*>(dy.data_ptr());
     const T* rp = reinterpret_cast<const T*>(r);
-    bwd_sums_kernel<T, V><<<grid, BLOCK, 0, stream>>>(
-        yp, xp, rp, st, gm, bt, pt, s.groups, s.cpg, (int)act, d);
-    bwd_join_kernel<<<joins, BLOCK, 0, stream>>>(
+    auto sums = [&](auto kernel) {
+      kernel<<<grid, BLOCK, 0, stream>>>(yp, xp, rp, mk, st, gm, bt, pt,
+                                         s.groups, s.cpg, d);
+    };
+    auto apply = [&](auto kernel) {
+      kernel<<<grid, BLOCK, 0, stream>>>(
+          yp, xp, rp, mk, st, gm, bt, gp, reinterpret_cast<T*>(dxp),
+          reinterpret_cast<T*>(drp), s.groups, s.cpg, d);
+    };
+    if (act == SILU) sums(bwd_sums_kernel<T, V, true>);
+    else sums(bwd_sums_kernel<T, V, false>);
+    bwd_join_kernel<<<joins, JOIN, 0, stream>>>(
         pt, gm, cp, gp, all, s.groups, s.cpg, across, d);
     params();
-    if (dxp || drp)
-      bwd_apply_kernel<T, V><<<grid, BLOCK, 0, stream>>>(
-          yp, xp, rp, st, gm, bt, gp, reinterpret_cast<T*>(dxp),
-          reinterpret_cast<T*>(drp), s.groups, s.cpg, (int)act, d);
+    if (dxp || drp) {
+      if (act == SILU) apply(bwd_apply_kernel<T, V, true>);
+      else apply(bwd_apply_kernel<T, V, false>);
+    }
   });
   return {dx, dres, dgamma, dbeta};
 }

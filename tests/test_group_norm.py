@@ -292,6 +292,29 @@ def test_gpu_constant_groups():
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("dtype", ["bf16", "fp32"])
+@pytest.mark.parametrize("shape,groups", [((2, 16, 16, 64), 8),
+                                          ((1, 150, 150, 16), 2)])
+def test_gpu_relu_gate_next_to_zero(shape, groups, dtype):
+    """The residual is chosen as minus what the norm gives, rounded: many z
+    are next to zero, where fp32 does not tell their sign. The gate is the
+    sign in 64 bits, but for those within 2e-8 of the terms: the mean adds
+    fp32 runs, each off by 2^-24 of itself, hundreds of them independent."""
+    x, gamma, beta, _, dy = inputs(*shape, dtype)
+    vals, _ = oracle(x, gamma, beta, None, dy, groups, "none")
+    res = (-vals["y"]).to(TYPES[dtype])
+    g = torch.Generator().manual_seed(1)
+    wide = torch.randn(shape, generator=g).to(TYPES[dtype])
+    res = torch.where(torch.rand(shape, generator=g) < 0.5, res, wide)
+    z = vals["y"] + res.double()
+    got = run_gpu(x, gamma, beta, res, dy, groups, "relu")["dres"].cpu()
+    want = torch.where(z > 0, dy.double(), 0.0)
+    sure = z.abs() > 2e-8 * (1 + res.double().abs())
+    assert int((~sure).sum()) < z.numel() // (2 if dtype == "fp32" else 1000)
+    assert torch.equal(got.double()[sure], want[sure])
+
+
+@pytest.mark.gpu
 def test_gpu_odd_alignment():
     """A view that starts in the middle of a 16-byte word."""
     n, h, w, c = 2, 5, 5, 16
@@ -308,6 +331,16 @@ def test_gpu_odd_alignment():
         a.requires_grad_(True)
         y = O.group_norm(a, gamma.to(DEV), beta.to(DEV), 4, 1e-5, "relu", r)
         y.backward(shifted(dy, by))
+        close("y", y, vals, sizes)
+        close("dx", a.grad, vals, sizes)
+    # and each of them alone
+    for at in range(3):
+        t = [x.to(DEV), res.to(DEV), dy.to(DEV)]
+        t[at] = shifted(t[at], 1)
+        a = t[0].requires_grad_(True)
+        y = O.group_norm(a, gamma.to(DEV), beta.to(DEV), 4, 1e-5, "relu",
+                         t[1])
+        y.backward(t[2])
         close("y", y, vals, sizes)
         close("dx", a.grad, vals, sizes)
 
