@@ -135,8 +135,8 @@ class AdamW:
         b1, b2 = (float(b) for b in betas)
         if not (0.0 <= b1 < 1.0 and 0.0 <= b2 < 1.0):
             raise ValueError(f"betas must be in [0, 1), got {betas}")
-        if not 2.0 ** -126 <= eps < math.inf:
-            raise ValueError(f"eps must be positive, got {eps}")
+        if not 1e-12 <= eps < math.inf:
+            raise ValueError(f"eps must be at least 1e-12, got {eps}")
         if not 0.0 <= weight_decay < math.inf:
             raise ValueError(f"weight_decay must not be negative, "
                              f"got {weight_decay}")

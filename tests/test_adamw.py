@@ -183,7 +183,7 @@ def test_small_second_moment_never_zero():
     zero; the step must stay a step."""
     space, _ = space_of([(64,)])
     before = space.param.clone()
-    opt = AdamW(space, lr=1e-3, weight_decay=0.0, state_bits=8, eps=1e-30)
+    opt = AdamW(space, lr=1e-3, weight_decay=0.0, state_bits=8, eps=1e-12)
     space.grad.fill_(1e-9)
     space.grad[0] = 1.0
     for _ in range(20):
@@ -366,7 +366,7 @@ def test_state_refusals():
 
 @pytest.mark.parametrize("kw", [
     dict(lr=-1.0), dict(lr=math.nan), dict(betas=(1.0, 0.9)),
-    dict(betas=(0.9, -0.1)), dict(eps=0.0), dict(eps=-1e-8),
+    dict(betas=(0.9, -0.1)), dict(eps=0.0), dict(eps=-1e-8), dict(eps=1e-13),
     dict(weight_decay=-1.0), dict(state_bits=16)])
 def test_refusals(kw):
     space, _ = space_of([(3,)])
