@@ -135,6 +135,28 @@ __device__ __forceinline__ unsigned max16(unsigned v) {
 
 // ---- the step -------------------------------------------------------------
 
+// Gradients and moments pass by: nothing reads them again before the next
+// step, and kept out of the caches they leave room for the weights, which the
+// next pass reads. On 17.4 M weights the 32-bit step takes 72 us so, and 91 us
+// without; the 8-bit step 52 and 56.
+template <typename T>
+__device__ __forceinline__ T pass_in(const T* p) {
+  static_assert(sizeof(T) == 16 || sizeof(T) == 8, "");
+  using W = std::conditional_t<sizeof(T) == 16, f32x4, unsigned long>;
+  const W w = __builtin_nontemporal_load(reinterpret_cast<const W*>(p));
+  T t;
+  __builtin_memcpy(&t, &w, sizeof(T));
+  return t;
+}
+
+template <typename T>
+__device__ __forceinline__ void pass_out(T* p, const T& t) {
+  using W = std::conditional_t<sizeof(T) == 16, f32x4, unsigned long>;
+  W w;
+  __builtin_memcpy(&w, &t, sizeof(T));
+  __builtin_nontemporal_store(w, reinterpret_cast<W*>(p));
+}
+
 // chunks: [start, length, tensor] each; a chunk starts at a multiple of QB
 // and is taken to the next one beyond its length: the gap behind a tensor
 // belongs to it, and zeros there stay zeros.
@@ -157,17 +179,17 @@ __global__ void __launch_bounds__(BLOCK) step_kernel(
   for (int i = threadIdx.x * 4; i < padded; i += BLOCK * 4) {
     const long at = start + i;
     float4 p = *reinterpret_cast<const float4*>(param + at);
-    const float4 g = *reinterpret_cast<const float4*>(grad + at);
+    const float4 g = pass_in(reinterpret_cast<const float4*>(grad + at));
     float4 m, v;
     float* pp = reinterpret_cast<float*>(&p);
     const float* gg = reinterpret_cast<const float*>(&g);
     float* mm = reinterpret_cast<float*>(&m);
     float* vv = reinterpret_cast<float*>(&v);
     if (BITS == 32) {
-      m = *reinterpret_cast<const float4*>(m32 + at);
-      v = *reinterpret_cast<const float4*>(v32 + at);
+      m = pass_in(reinterpret_cast<const float4*>(m32 + at));
+      v = pass_in(reinterpret_cast<const float4*>(v32 + at));
     } else {
-      decode4(codes[at >> 2], exps[at / QB], mm, vv);
+      decode4(pass_in(codes + (at >> 2)), exps[at / QB], mm, vv);
     }
     unsigned top_m = 0, top_v = 0;
 #pragma unroll
@@ -181,8 +203,8 @@ __global__ void __launch_bounds__(BLOCK) step_kernel(
     }
     *reinterpret_cast<float4*>(param + at) = p;
     if (BITS == 32) {
-      *reinterpret_cast<float4*>(m32 + at) = m;
-      *reinterpret_cast<float4*>(v32 + at) = v;
+      pass_out(reinterpret_cast<float4*>(m32 + at), m);
+      pass_out(reinterpret_cast<float4*>(v32 + at), v);
     } else {
       // 16 lanes hold one block of 64, and all of them are here: chunks are
       // cut and padded in whole blocks
@@ -201,7 +223,7 @@ __global__ void __launch_bounds__(BLOCK) step_kernel(
         code.x |= qm << (8 * j);
         code.y |= qv << (8 * j);
       }
-      codes[at >> 2] = code;
+      pass_out(codes + (at >> 2), code);
       if ((threadIdx.x & 15) == 0)
         exps[at / QB] = make_uchar2((unsigned char)em, (unsigned char)ev);
     }
@@ -218,19 +240,26 @@ __global__ void __launch_bounds__(BLOCK) step_kernel(
   }
 }
 
-// one wave a tensor: its chunks' parts, added in a fixed order. The first
+// one block a tensor: its chunks' parts, added in a fixed order. The first
 // block moves the step on.
-__global__ void __launch_bounds__(64) finish_kernel(
+constexpr int FINISH = 512;
+__global__ void __launch_bounds__(FINISH) finish_kernel(
     const float* __restrict__ part, const long* __restrict__ first,
     float* __restrict__ norms, float* __restrict__ coef,
     long* __restrict__ step, double b1, double b2) {
   const long a = first[blockIdx.x], b = first[blockIdx.x + 1];
   float acc = 0.f;
-  for (long i = a + threadIdx.x; i < b; i += 64) acc += part[i];
+#pragma unroll 8
+  for (long i = a + threadIdx.x; i < b; i += FINISH) acc += part[i];
 #pragma unroll
   for (int d = 32; d; d >>= 1) acc += __shfl_xor(acc, d);
+  __shared__ float waves[FINISH / 64];
+  if ((threadIdx.x & 63) == 0) waves[threadIdx.x >> 6] = acc;
+  __syncthreads();
   if (threadIdx.x == 0) {
-    norms[blockIdx.x] = acc;
+    float s = 0.f;
+    for (int w = 0; w < FINISH / 64; ++w) s += waves[w];
+    norms[blockIdx.x] = s;
     if (blockIdx.x == 0) {
       const long t = step[0] + 1;
       step[0] = t;
@@ -329,7 +358,7 @@ torch::Tensor adamw_step_norm(torch::Tensor param, torch::Tensor grad,
   if (k) {
     if (bits8) run(step_kernel<8>); else run(step_kernel<32>);
   }
-  finish_kernel<<<(unsigned)sz, 64, 0, cur_stream()>>>(
+  finish_kernel<<<(unsigned)sz, FINISH, 0, cur_stream()>>>(
       part.data_ptr<float>(), first.data_ptr<long>(),
       norms.data_ptr<float>(), coef.data_ptr<float>(), step.data_ptr<long>(),
       b1, b2);

@@ -30,7 +30,10 @@ from ..ops.backend import native
 from .flat import ALIGN, FlatParamSpace
 
 QBLOCK = 64       # values that share an exponent; divides ALIGN
-CHUNK = 4096      # values of one kernel block; a multiple of QBLOCK
+# Values of one kernel block, a multiple of QBLOCK: four a thread, none of
+# which then waits behind another. The 8-bit step of 17.4 M weights took 56 us
+# with 1,024, 62 us with 4,096 and 68 us with 16,384.
+CHUNK = 1024
 
 assert ALIGN % QBLOCK == 0 and CHUNK % QBLOCK == 0
 
