@@ -23,8 +23,8 @@ torch::Tensor trigger_decide(torch::Tensor, torch::Tensor, torch::Tensor,
 torch::Tensor adamw_step_norm(torch::Tensor, torch::Tensor, torch::Tensor,
                               torch::Tensor, torch::Tensor, torch::Tensor,
                               torch::Tensor, torch::Tensor, torch::Tensor,
-                              torch::Tensor, torch::Tensor, double, double,
-                              double, long);
+                              torch::Tensor, torch::Tensor, torch::Tensor,
+                              torch::Tensor, double, double, double, long);
 std::vector<torch::Tensor> adamw_moments(torch::Tensor, torch::Tensor);
 // elementwise.hip
 torch::Tensor relu_fwd(torch::Tensor);

@@ -176,7 +176,11 @@ class AdamW:
         self._chunks = torch.tensor(rows, **i64).reshape(-1, 3)
         self._first = torch.tensor(first, **i64)
         self._step = torch.zeros(1, **i64)
+        # scratch of the norms, and behind it a counter that ends at zero
+        self._part = torch.zeros(len(rows) + 1, **f32)
+        # of the next step: lr, 1 / (1 - b1^t), 1 / sqrt(1 - b2^t); b1^t, b2^t
         self._coef = torch.zeros(3, **f32)
+        self._powers = torch.zeros(2, dtype=torch.float64, device=dev)
         self.lr = lr
         self._set_corrections(1)
 
@@ -199,9 +203,10 @@ class AdamW:
 
     def _set_corrections(self, t: int) -> None:
         """Those of step t, which is the next."""
-        b1, b2 = self.betas
-        self._coef[1] = 1.0 / (1.0 - b1 ** t)
-        self._coef[2] = 1.0 / math.sqrt(1.0 - b2 ** t)
+        p1, p2 = (b ** t for b in self.betas)
+        self._powers.copy_(torch.tensor([p1, p2], dtype=torch.float64))
+        self._coef[1:].copy_(torch.tensor(
+            [1.0 / (1.0 - p1), 1.0 / math.sqrt(1.0 - p2)]))
 
     # -- the step ------------------------------------------------------------
     def step(self) -> torch.Tensor:
@@ -210,8 +215,8 @@ class AdamW:
             return native().adamw_step_norm(
                 sp.param, sp.grad, self.exp_avg, self.exp_avg_sq, self.codes,
                 self.exponents, self._chunks, self._first, self._decay,
-                self._coef, self._step, self.betas[0], self.betas[1],
-                self.eps, self.seed)
+                self._coef, self._powers, self._step, self._part,
+                self.betas[0], self.betas[1], self.eps, self.seed)
         return self._step_cpu()
 
     def _step_cpu(self) -> torch.Tensor:

@@ -225,7 +225,11 @@ def test_extreme_sizes(device):
 
 @pytest.mark.gpu
 @pytest.mark.parametrize("shapes", [SHAPES, [(1,)], [(3, 3)] * 300,
-                                    [(70000,), (4097, 5)]], ids=len)
+                                    [(70000,), (4097, 5)],
+                                    [(255 * 1024, 1), (5,)],   # 256 chunks
+                                    [(256 * 1024,), (5, 7)],   # 257
+                                    [(3, 1000)] * 400],
+                         ids=lambda s: f"{len(s)}x{s[0]}")
 def test_gpu_8_bits_equal_cpu(shapes):
     """The codes are the CPU's to the bit, step after step: what decides them
     is rounded after each operation on both sides. The weights are off by the
