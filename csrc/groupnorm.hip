@@ -3,74 +3,99 @@
 namespace eg {
 namespace gn {
 
+// values of a group in `rows` rows of a slab: the group's, or where a slice
+// is one of several in a group those of slice `sub`
+__device__ __forceinline__ double piece(const Slab& d, int v, int rows,
+                                        int sub) {
+  const int wide = d.span * v == d.cpg
+                       ? min(d.lanes, d.span - sub * d.lanes) * v
+                       : d.cpg;
+  return (double)rows * wide;
+}
+
 // ---- forward --------------------------------------------------------------
 
-// Each channel's mean and sum of squared distances from it over one chunk of
-// rows. Distances are first measured from the chunk's own first value, which
-// is among those it adds, so that a large mean costs no digits.
-template <typename T, int V>
+// Each group's mean and sum of squared distances from it over one chunk of
+// rows. Distances are first measured from the group's first value in the
+// chunk, which is among those added, so that a large mean costs no digits.
+template <typename T, int V, int P>
 __global__ void __launch_bounds__(BLOCK) stats_kernel(
-    const T* __restrict__ x, float2* __restrict__ part, Deal d) {
-  __shared__ float slot[BLOCK / 2 * 2 * V];
-  const Place at(d);
-  float from[V] = {}, sums[2 * V] = {};
-  if (at.on) {
-    const T* xs = x + ((long)at.n * d.hw + at.begin) * d.c + at.col * V;
-    const Vec<T, V> f = load<T, V>(xs);
-#pragma unroll
-    for (int j = 0; j < V; ++j) from[j] = (float)f.v[j];
+    const T* __restrict__ x, float2* __restrict__ part_of, Slab d) {
+  __shared__ float table[2 * BLOCK * P];
+  __shared__ float from_of[BLOCK];
+  const Spot at(d, V);
+  // entries of a group: its slices, and the chunks of each
+  const bool alone = d.span * V == d.cpg;
+  const int unit = d.by_subs.of(at.slice);
+  const int subs = alone ? d.subs : 1;
+  const int sub = alone ? at.slice - unit * d.subs : 0;
+  const int group = alone ? unit : at.slice * d.in_slice;
+  const T* row0 = x + ((long)at.n * d.hw + at.begin) * d.c;
+  float from[P], s[P] = {}, q2[P] = {};
+  each_part<P>(alone ? 0 : at.lane * V, d, [&](int j, int q) {
+    from[j] = (float)row0[(long)(group + q) * d.cpg];
+  });
+  const int steps = (at.count + d.rows - 1) / d.rows;
 #pragma unroll 4
-    for (int k = at.r; k < at.count; k += d.rows) {
-      const Vec<T, V> a = load<T, V>(xs + (long)k * d.c);
+  for (int k = 0; k < steps; ++k) {
+    if (at.has(k, d)) {
+      const Vec<T, V> a = load<T, V>(at.row(x, k));
 #pragma unroll
       for (int j = 0; j < V; ++j) {
-        const float e = (float)a.v[j] - from[j];
-        sums[j] += e;
-        sums[V + j] = fmaf(e, e, sums[V + j]);
+        const int p = P == 1 ? 0 : j;
+        const float e = a[j] - from[p];
+        s[p] += e;
+        q2[p] = fmaf(e, e, q2[p]);
       }
     }
   }
-  add_rows<2 * V>(sums, slot, at.r, at.lane, d.lanes, d.rows);
-  if (at.on && at.r == 0) {
-    float2* to = part + (long)blockIdx.x * d.c + at.col * V;
-    const float inv = 1.f / (float)at.count;
 #pragma unroll
-    for (int j = 0; j < V; ++j) {
-      const float off = sums[j] * inv;
-      to[j] = make_float2(from[j] + off, fmaf(-sums[j], off, sums[V + j]));
-    }
+  for (int j = 0; j < P; ++j) {
+    table[j * blockDim.x + threadIdx.x] = s[j];
+    table[(P + j) * blockDim.x + threadIdx.x] = q2[j];
   }
+  for (int q = threadIdx.x; q < d.in_slice; q += blockDim.x)
+    from_of[q] = (float)row0[(long)(group + q) * d.cpg];
+  __syncthreads();
+  const int rows = fold<2 * P>(table, d, P == 1 ? BLOCK : 8);
+  const double values = piece(d, V, at.count, sub);
+  add_groups<Twice>(
+      rows, d,
+      [&](int e, int row) {
+        return Twice{part<P>(table, d, e, row),
+                     part<P>(table + P * blockDim.x, d, e, row)};
+      },
+      [&](int q, const Twice& t) {
+        const double off = t.a / values;
+        part_of[(((long)at.n * d.groups + group + q) * subs + sub) * d.chunks +
+                at.chunk] =
+            make_float2((float)(from_of[q] + off), (float)(t.b - t.a * off));
+      });
 }
 
-// One block a group: joins the channels and chunks of each,
+// Joins the pieces of each group, a block for each,
 //   M2 = sum (M2_i + count_i mean_i^2) - M mean^2,
 // which in 64 bits leaves 16 digits less those of (mean / spread)^2.
 // Mean and rstd are kept in 64 bits: the sign of z decides a ReLU's gradient,
 // and where z is next to zero it is computed again from them.
-__global__ void __launch_bounds__(JOIN) join_kernel(
+__global__ void __launch_bounds__(BLOCK) join_kernel(
     const float2* __restrict__ part, double2* __restrict__ stats, long groups,
-    int per_sample, int cpg, Deal d, double eps) {
-  __shared__ double slot[JOIN / 64];
-  const int entries = d.chunks * cpg;
-  const int down = JOIN / cpg, right = JOIN % cpg;
-  const double m = (double)d.hw * cpg;
+    int v, Slab d, double eps) {
+  __shared__ double slot[BLOCK / 64];
+  const bool alone = d.span * v == d.cpg;
+  const int subs = alone ? d.subs : 1;
+  const double m = (double)d.hw * d.cpg;
   for (long g = blockIdx.x; g < groups; g += gridDim.x) {
-    const float2* p = part + g / per_sample * d.chunks * d.c +
-                      g % per_sample * cpg;
+    const float2* p = part + g * subs * d.chunks;
     double s = 0, q = 0;
-    int chunk = threadIdx.x / cpg, ch = threadIdx.x % cpg;
-#pragma unroll 4
-    for (int i = threadIdx.x; i < entries; i += JOIN) {
-      const float2 e = p[(long)chunk * d.c + ch];
-      const double rows = min(d.per_chunk, d.hw - chunk * d.per_chunk);
-      s += rows * e.x;
-      q += (double)e.y + rows * e.x * e.x;
-      chunk += down;
-      ch += right;
-      if (ch >= cpg) {
-        ch -= cpg;
-        ++chunk;
-      }
+    for (int i = threadIdx.x; i < subs * d.chunks; i += blockDim.x) {
+      const int chunk = i % d.chunks;
+      const double n =
+          piece(d, v, min(d.per_chunk, d.hw - chunk * d.per_chunk),
+                i / d.chunks);
+      const float2 e = p[i];
+      s += n * e.x;
+      q += (double)e.y + n * e.x * e.x;
     }
     const double mean = add_block(s, slot) / m;
     const double var = add_block(q, slot) / m - mean * mean;
@@ -120,97 +145,69 @@ __global__ void __launch_bounds__(BLOCK) apply_kernel(
   }
 }
 
-// The slab in one pass. P: statistics that a thread needs, 1 where a vector
-// lies within a group, else one a channel.
+// All of it in one pass over a slab of whole samples.
 template <typename T, int V, int I, int P, int ACT>
-__global__ void __launch_bounds__(SLAB) slab_kernel(
+__global__ void __launch_bounds__(I <= WIDE_VECTORS ? SLAB : SPAN) slab_kernel(
     const T* __restrict__ x, const T* __restrict__ res, T* __restrict__ y,
     unsigned char* __restrict__ mask, double2* __restrict__ stats,
     const float* __restrict__ gamma, const float* __restrict__ beta,
     double eps, Slab d) {
-  __shared__ float table[SLAB * P];
-  __shared__ double mean_of[SLAB];
-  __shared__ double rstd_of[SLAB];
+  __shared__ float table[(I <= WIDE_VECTORS ? SLAB : SPAN) * P];
+  __shared__ double mean_of[SPAN];
+  __shared__ double rstd_of[SPAN];
   const Spot at(d, V);
-  const int w = P == 1 ? d.cpg / V : d.cpg;
-  const double m = (double)d.hw * d.cpg;
-  const long base = (long)at.n * d.hw * d.c + at.first + at.lane * V;
   Vec<T, V> a[I];
 #pragma unroll
-  for (int k = 0; k < I; ++k) {
-    const int row = at.r + k * d.rows;
-    if (at.on && row < d.hw) a[k] = load<T, V>(x + base + (long)row * d.c);
-  }
-  float s[P] = {};
-#pragma unroll
-  for (int k = 0; k < I; ++k) {
-    if (at.on && at.r + k * d.rows < d.hw) {
-#pragma unroll
-      for (int j = 0; j < V; ++j) s[P == 1 ? 0 : j] += (float)a[k].v[j];
-    }
-  }
-#pragma unroll
-  for (int j = 0; j < P; ++j) table[threadIdx.x * P + j] = s[j];
-  __syncthreads();
-  add_groups<double>(table, d.rows, w, d,
-                     [&](int q, double t) { mean_of[q] = t / m; });
-  __syncthreads();
-  float mean[P];
-#pragma unroll
-  for (int j = 0; j < P; ++j) {
-    mean[j] = (float)mean_of[(at.lane * V + j) / d.cpg];
-    s[j] = 0.f;
-  }
-#pragma unroll
-  for (int k = 0; k < I; ++k) {
-    if (at.on && at.r + k * d.rows < d.hw) {
-#pragma unroll
-      for (int j = 0; j < V; ++j) {
-        const int p = P == 1 ? 0 : j;
-        const float e = (float)a[k].v[j] - mean[p];
-        s[p] = fmaf(e, e, s[p]);
-      }
-    }
-  }
-#pragma unroll
-  for (int j = 0; j < P; ++j) table[threadIdx.x * P + j] = s[j];
-  __syncthreads();
-  add_groups<double>(table, d.rows, w, d, [&](int q, double t) {
-    const double rstd = 1.0 / sqrt(t / m + eps);
-    rstd_of[q] = rstd;
-    if (stats)
-      stats[(long)at.n * d.groups + at.first / d.cpg + q] =
-          make_double2(mean_of[q], rstd);
-  });
-  __syncthreads();
-  if (!at.on) return;
-  const int c0 = at.first + at.lane * V;
-  float scale[V], shift[V], limit = 0.f;
+  for (int k = 0; k < I; ++k)
+    if (at.has(k, d)) a[k] = load<T, V>(at.row(x, k));
+  const int c0 = at.first;
+  float scale[V], shift[V], mean[P];
 #pragma unroll
   for (int j = 0; j < V; ++j) {
-    const int p = P == 1 ? 0 : j;
-    scale[j] = (float)(gamma[c0 + j] * rstd_of[(at.lane * V + p) / d.cpg]);
+    scale[j] = gamma[c0 + j];
     shift[j] = beta[c0 + j];
-    limit = fmaxf(limit, fabsf(scale[j] * mean[p]) + 2.f * fabsf(shift[j]));
   }
+  statistics<T, V, I, P>(
+      a, at, d, table, mean_of, mean, [&](int q, double mu, double m2) {
+        const double rstd = 1.0 / sqrt(m2 * d.inv + eps);
+        rstd_of[q] = rstd;
+        if (stats)
+          stats[(long)at.n * d.groups + at.slice * d.in_slice + q] =
+              make_double2(mu, rstd);
+      });
+  if (!at.on) return;
+  float limit = 0.f;
+  if (P == 1) {
+    const double rstd = rstd_of[d.by_cpg.of(at.lane * V)];
+#pragma unroll
+    for (int j = 0; j < V; ++j) scale[j] = (float)(scale[j] * rstd);
+  } else {
+    each_part<P>(at.lane * V, d, [&](int j, int q) {
+      scale[j] = (float)(scale[j] * rstd_of[q]);
+    });
+  }
+#pragma unroll
+  for (int j = 0; j < V; ++j)
+    limit = fmaxf(limit, fabsf(scale[j] * mean[P == 1 ? 0 : j]) +
+                             2.f * fabsf(shift[j]));
   limit *= 0x1p-20f;
 #pragma unroll
   for (int k = 0; k < I; ++k) {
-    const int row = at.r + k * d.rows;
-    if (row >= d.hw) break;
-    const long i = base + (long)row * d.c;
+    if (!at.has(k, d)) break;
+    renew<T, V>(a[k]);
     Vec<T, V> b;
-    if (res) b = load<T, V>(res + i);
+    if (res) b = load<T, V>(at.row(res, k));
     auto exact = [&](int j) {
       const int q = (at.lane * V + j) / d.cpg;
-      const double z = ((double)(float)x[i + j] - mean_of[q]) * rstd_of[q] *
-                           (double)gamma[c0 + j] + (double)beta[c0 + j];
-      return res ? z + (double)(float)res[i + j] : z;
+      const double z = ((double)(float)at.row(x, k)[j] - mean_of[q]) *
+                           rstd_of[q] * (double)gamma[c0 + j] +
+                       (double)beta[c0 + j];
+      return res ? z + (double)(float)at.row(res, k)[j] : z;
     };
     const unsigned bits = activate<T, V, P, ACT>(a[k], b, res, mean, scale,
                                                  shift, limit, exact);
-    store<T, V>(y + i, a[k]);
-    if (ACT == RELU_BITS) mask[i / V] = (unsigned char)bits;
+    store<T, V>(at.row(y, k), a[k]);
+    if (ACT == RELU_BITS) *at.template bits<V>(mask, k) = (unsigned char)bits;
   }
 }
 
@@ -241,7 +238,7 @@ static torch::Tensor forward(const torch::Tensor& x,
     mk = mask->data_ptr<unsigned char>();
   }
   const hipStream_t stream = cur_stream();
-  const Cut slab = cut(s, v, size, FWD_VECTORS);
+  const Cut slab = cut(s, v, size, SLAB, FWD_VECTORS, false);
   if (slab.threads) {
     auto* st = stats ? reinterpret_cast<double2*>(stats->data_ptr()) : nullptr;
     with_slab(x.scalar_type(), v, slab.vectors, s.cpg % v == 0, [&](auto tag) {
@@ -261,27 +258,43 @@ static torch::Tensor forward(const torch::Tensor& x,
     return y;
   }
   torch::Tensor own = stats ? *stats : torch::empty({s.n, s.groups, 2}, f64);
-  const Deal d = deal(s.hw, s.c, v, s.n);
-  auto part = torch::empty({s.n, d.chunks, s.c, 2},
+  int vs = v;       // of the statistics, which may have to be narrower
+  const Cut chunk = chop(s, vs, true);
+  const Slab& cd = chunk.d;
+  const int subs = cd.span * vs == s.cpg ? cd.subs : 1;
+  auto part = torch::empty({s.n * s.groups * subs * cd.chunks, 2},
                            x.options().dtype(torch::kFloat32));
+  const Deal d = deal(s.hw, s.c, v, s.n);
   const dim3 grid((unsigned)(s.n * d.chunks), 1,
                   (unsigned)((d.cols + d.lanes - 1) / d.lanes));
   const long all = s.n * s.groups;
   const unsigned joins = (unsigned)std::min<long>(all, 1 << 20);
+  const long blocks = s.n * cd.slices * cd.chunks;
+  TORCH_CHECK(blocks < (1L << 24), "group_norm: the input is too large");
   auto* st = reinterpret_cast<double2*>(own.data_ptr());
   auto* pt = reinterpret_cast<float2*>(part.data_ptr());
-  with_type(x.scalar_type(), v, [&](auto tag) {
+  const auto type = x.scalar_type();
+  const bool inside = s.cpg % vs == 0;
+  with_type(type, vs, [&](auto tag) {
     using T = typename decltype(tag)::type;
     constexpr int V = decltype(tag)::v;
-    const T* xp = reinterpret_cast<const T*>(x.data_ptr());
-    stats_kernel<T, V><<<grid, BLOCK, 0, stream>>>(xp, pt, d);
-    join_kernel<<<joins, JOIN, 0, stream>>>(pt, st, all, s.groups, s.cpg, d,
-                                             eps);
+    auto run = [&](auto kernel) {
+      kernel<<<(unsigned)blocks, chunk.threads, 0, stream>>>(
+          reinterpret_cast<const T*>(x.data_ptr()), pt, cd);
+    };
+    if (inside) run(stats_kernel<T, V, 1>);
+    else run(stats_kernel<T, V, V>);
+  });
+  const int join = subs * cd.chunks > 64 ? BLOCK : 64;
+  join_kernel<<<joins, join, 0, stream>>>(pt, st, all, vs, cd, eps);
+  with_type(type, v, [&](auto tag) {
+    using T = typename decltype(tag)::type;
+    constexpr int V = decltype(tag)::v;
     with_act(act, mk, [&](auto a) {
       apply_kernel<T, V, decltype(a)::v><<<grid, BLOCK, 0, stream>>>(
-          xp, reinterpret_cast<const T*>(r),
-          reinterpret_cast<T*>(y.data_ptr()), mk, st, gm, bt, s.groups, s.cpg,
-          d);
+          reinterpret_cast<const T*>(x.data_ptr()),
+          reinterpret_cast<const T*>(r), reinterpret_cast<T*>(y.data_ptr()),
+          mk, st, gm, bt, s.groups, s.cpg, d);
     });
   });
   return y;

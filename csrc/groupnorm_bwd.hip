@@ -5,85 +5,50 @@ namespace gn {
 
 // ---- backward -------------------------------------------------------------
 
-// What a thread keeps of its V channels. SILU: dz is dy times the slope at z;
-// without, it is dy where the forward pass left a bit, or everywhere.
-template <typename T, int V, bool SILU_>
-struct Channels {
-  float mean[V], rstd[V], gamma[V], beta[SILU_ ? V : 1];
+// dz / dy of a SiLU at z
+__device__ __forceinline__ float silu_slope(float z) {
+  const float s = sigmoid(z);
+  return s * fmaf(z, 1.f - s, 1.f);
+}
 
-  __device__ __forceinline__ Channels(const double2* sample, int c0,
-                                      const float* g, const float* b,
-                                      int cpg) {
+// What a thread keeps of its V channels where sums are applied. SILU: dz is dy
+// times the slope at z; without, it is dy where the forward pass left a bit,
+// or everywhere.
+template <typename T, int V, bool SILU_>
+struct Applied {
+  float mean[V], rstd[V], scale[V], shift[SILU_ ? V : 1];
+
+  __device__ __forceinline__ Applied(const double2* sample, int c0,
+                                     const float* gamma, const float* beta,
+                                     int cpg) {
 #pragma unroll
     for (int j = 0; j < V; ++j) {
       const double2 st = sample[(c0 + j) / cpg];
       mean[j] = (float)st.x;
       rstd[j] = (float)st.y;
-      gamma[j] = g[c0 + j];
-      if (SILU_) beta[j] = b[c0 + j];
+      scale[j] = gamma[c0 + j] * rstd[j];
+      if (SILU_) shift[j] = beta[c0 + j];
     }
   }
 
-  __device__ __forceinline__ float dz(int j, float xh, float r,
+  __device__ __forceinline__ float dz(int j, float off, float r,
                                       float dy) const {
     if (!SILU_) return dy;
-    const float z = fmaf(xh, gamma[j], beta[j]) + r;
-    const float s = sigmoid(z);
-    return dy * (s * fmaf(z, 1.f - s, 1.f));
+    return dy * silu_slope(fmaf(off, scale[j], shift[j]) + r);
   }
 };
 
-// Each channel's sums of dz and of dz xh over one chunk of rows.
-template <typename T, int V, bool SILU_>
-__global__ void __launch_bounds__(BLOCK) bwd_sums_kernel(
-    const T* __restrict__ dy, const T* __restrict__ x,
-    const T* __restrict__ res, const unsigned char* __restrict__ mask,
-    const double2* __restrict__ stats, const float* __restrict__ gamma,
-    const float* __restrict__ beta, float2* __restrict__ part, int groups,
-    int cpg, Deal d) {
-  __shared__ float slot[BLOCK / 2 * 2 * V];
-  const Place at(d);
-  float sums[2 * V] = {};
-  if (at.on) {
-    const Channels<T, V, SILU_> ch(stats + (long)at.n * groups, at.col * V,
-                                   gamma, beta, cpg);
-    const long base = ((long)at.n * d.hw + at.begin) * d.c + at.col * V;
-#pragma unroll 2
-    for (int k = at.r; k < at.count; k += d.rows) {
-      const long i = base + (long)k * d.c;
-      const Vec<T, V> a = load<T, V>(x + i);
-      Vec<T, V> g = load<T, V>(dy + i), b;
-      if (SILU_ && res) b = load<T, V>(res + i);
-      if (!SILU_ && mask) keep<T, V>(g, mask[i / V]);
-#pragma unroll
-      for (int j = 0; j < V; ++j) {
-        const float xh = ((float)a.v[j] - ch.mean[j]) * ch.rstd[j];
-        const float dz = ch.dz(j, xh, SILU_ && res ? (float)b.v[j] : 0.f,
-                               (float)g.v[j]);
-        sums[j] += dz;
-        sums[V + j] = fmaf(dz, xh, sums[V + j]);
-      }
-    }
-  }
-  add_rows<2 * V>(sums, slot, at.r, at.lane, d.lanes, d.rows);
-  if (at.on && at.r == 0) {
-    float2* to = part + (long)blockIdx.x * d.c + at.col * V;
-#pragma unroll
-    for (int j = 0; j < V; ++j) to[j] = make_float2(sums[j], sums[V + j]);
-  }
-}
-
-// One block a group: each channel's sums over the chunks, for dgamma and
-// dbeta, and the group's s1 and s2.
+// A block a group: each channel's sums over the chunks, for dgamma and dbeta,
+// and the group's s1 and s2.
 __global__ void __launch_bounds__(JOIN) bwd_join_kernel(
     const float2* __restrict__ part, const float* __restrict__ gamma,
     float2* __restrict__ channel, float2* __restrict__ group, long groups,
-    int per_sample, int cpg, int across, Deal d) {
+    int per_sample, int cpg, int across, Slab d) {
   // across: threads side by side over channels, a power of two
   __shared__ float2 slot[JOIN];
   __shared__ float sums[JOIN / 64];
-  const int lane = threadIdx.x % across, share = threadIdx.x / across;
-  const int shares = JOIN / across;
+  const int lane = threadIdx.x & (across - 1);
+  const int share = threadIdx.x / across, shares = blockDim.x / across;
   const float inv = 1.f / ((float)d.hw * (float)cpg);
   for (long g = blockIdx.x; g < groups; g += gridDim.x) {
     const long n = g / per_sample;
@@ -140,8 +105,8 @@ __global__ void __launch_bounds__(PC* PN) bwd_params_kernel(
       s += Pair{e.x, e.y};
     }
   }
-  s += across(s, 16);
-  s += across(s, 32);
+  s += across<16>(s);
+  s += across<32>(s);
   if (threadIdx.x % 64 < PC) slot[threadIdx.x / 64][lane] = s;
   __syncthreads();
   if (threadIdx.x < PC && ch < c) {
@@ -162,14 +127,15 @@ __global__ void __launch_bounds__(BLOCK) bwd_apply_kernel(
     T* __restrict__ dx, T* __restrict__ dres, int groups, int cpg, Deal d) {
   const Place at(d);
   if (!at.on) return;
-  const Channels<T, V, SILU_> ch(stats + (long)at.n * groups, at.col * V,
+  const Applied<T, V, SILU_> ch(stats + (long)at.n * groups, at.col * V,
                                  gamma, beta, cpg);
-  float s1[V], s2[V];
+  // dx = (rstd gamma) dz - (rstd^2 s2) (x - mean) - rstd s1
+  float by_x[V], less[V];
 #pragma unroll
   for (int j = 0; j < V; ++j) {
     const float2 s = group[(long)at.n * groups + (at.col * V + j) / cpg];
-    s1[j] = s.x;
-    s2[j] = s.y;
+    by_x[j] = -ch.rstd[j] * ch.rstd[j] * s.y;
+    less[j] = -ch.rstd[j] * s.x;
   }
   const long base = ((long)at.n * d.hw + at.begin) * d.c + at.col * V;
 #pragma unroll 2
@@ -179,142 +145,205 @@ __global__ void __launch_bounds__(BLOCK) bwd_apply_kernel(
     Vec<T, V> g = load<T, V>(dy + i), b, u;
     if (SILU_ && res) b = load<T, V>(res + i);
     if (!SILU_ && mask) keep<T, V>(g, mask[i / V]);
+    float dz[V], out[V];
 #pragma unroll
     for (int j = 0; j < V; ++j) {
-      const float xh = ((float)a.v[j] - ch.mean[j]) * ch.rstd[j];
-      const float dz = ch.dz(j, xh, SILU_ && res ? (float)b.v[j] : 0.f,
-                             (float)g.v[j]);
-      u.v[j] = (T)(ch.rstd[j] *
-                   (fmaf(dz, ch.gamma[j], -s1[j]) - xh * s2[j]));
-      if (SILU_) g.v[j] = (T)dz;
+      const float off = a[j] - ch.mean[j];
+      dz[j] = ch.dz(j, off, SILU_ && res ? b[j] : 0.f, g[j]);
+      out[j] = fmaf(dz[j], ch.scale[j], fmaf(off, by_x[j], less[j]));
     }
+    u.put(out);
+    if (SILU_) g.put(dz);
     if (dx) store<T, V>(dx + i, u);
     if (dres) store<T, V>(dres + i, g);
   }
 }
 
-// The slab in one pass: x and dy stay in registers between the sums and dx.
+// What a thread keeps of its channels, and dz from it. SILU: dz is dy times the
+// slope at z; without, it is dy where the forward pass left a bit, or
+// everywhere. P: parts of a vector with a mean of their own.
+template <typename T, int V, int P, bool SILU_>
+struct Channels {
+  float mean[P], rstd[P], scale[V], shift[SILU_ ? V : 1];
+
+  __device__ __forceinline__ Channels(const Spot& at, const Slab& d,
+                                      const double2* __restrict__ stats,
+                                      const float* __restrict__ gamma,
+                                      const float* __restrict__ beta) {
+    const double2* sample = stats + (long)at.n * d.groups;
+    each_part<P>(at.first, d, [&](int j, int q) {
+      const double2 st = sample[q];
+      mean[j] = (float)st.x;
+      rstd[j] = (float)st.y;
+    });
+#pragma unroll
+    for (int j = 0; j < V; ++j) {
+      scale[j] = gamma[at.first + j] * rstd[P == 1 ? 0 : j];
+      if (SILU_) shift[j] = beta[at.first + j];
+    }
+  }
+
+  __device__ __forceinline__ float off(int j, const Vec<T, V>& a) const {
+    return a[j] - mean[P == 1 ? 0 : j];
+  }
+
+  __device__ __forceinline__ float slope(int j, float off, float r) const {
+    return silu_slope(fmaf(off, scale[j], shift[j]) + r);
+  }
+
+  // adds a vector to the sums of dz and dz (x - mean), and leaves dz in b
+  // where a SiLU makes it
+  __device__ __forceinline__ void add(const Vec<T, V>& a, const Vec<T, V>& g,
+                                      Vec<T, V>& b, bool res,
+                                      float (&s)[2 * V]) const {
+    float dz[V];
+#pragma unroll
+    for (int j = 0; j < V; ++j) {
+      const float o = off(j, a);
+      dz[j] = g[j];
+      if (SILU_) dz[j] *= slope(j, o, res ? b[j] : 0.f);
+      s[j] += dz[j];
+      s[V + j] = fmaf(dz[j], o, s[V + j]);
+    }
+    if (SILU_) b.put(dz);
+  }
+
+  // the block's sums of dz and dz xh of each channel, in the table's first row
+  __device__ __forceinline__ void join(const float (&s)[2 * V], float* table,
+                                       const Slab& d) const {
+#pragma unroll
+    for (int j = 0; j < V; ++j) {
+      table[j * blockDim.x + threadIdx.x] = s[j];
+      table[(V + j) * blockDim.x + threadIdx.x] =
+          s[V + j] * rstd[P == 1 ? 0 : j];
+    }
+    __syncthreads();
+    fold<2 * V>(table, d, 1);
+  }
+};
+
+// One vector after the other: the scheduler would else work on all of a
+// thread's at once, with registers for as many.
+// (A SiLU may have the residual to load for each.)
+template <bool SILU_>
+__device__ __forceinline__ void in_turn() {
+  if (!SILU_) __builtin_amdgcn_sched_barrier(0);
+}
+
+template <int V>
+__device__ __forceinline__ Pair sums_of(const float* table, int c) {
+  return {table[c % V * blockDim.x + c / V],
+          table[(V + c % V) * blockDim.x + c / V]};
+}
+
+// Each channel's sums over one chunk of rows.
+template <typename T, int V, int P, bool SILU_>
+__global__ void __launch_bounds__(BLOCK) bwd_sums_kernel(
+    const T* __restrict__ dy, const T* __restrict__ x,
+    const T* __restrict__ res, const unsigned char* __restrict__ mask,
+    const double2* __restrict__ stats, const float* __restrict__ gamma,
+    const float* __restrict__ beta, float2* __restrict__ part, Slab d) {
+  __shared__ float table[2 * BLOCK * V];
+  const Spot at(d, V);
+  const Channels<T, V, P, SILU_> ch(at, d, stats, gamma, beta);
+  float s[2 * V] = {};
+  const int steps = (at.count + d.rows - 1) / d.rows;
+#pragma unroll 2
+  for (int k = 0; k < steps; ++k) {
+    if (at.has(k, d)) {
+      const Vec<T, V> a = load<T, V>(at.row(x, k));
+      Vec<T, V> g = load<T, V>(at.row(dy, k)), b;
+      if (SILU_ && res) b = load<T, V>(at.row(res, k));
+      if (!SILU_ && mask) keep<T, V>(g, *at.template bits<V>(mask, k));
+      ch.add(a, g, b, res, s);
+    }
+  }
+  ch.join(s, table, d);
+  const int c0 = at.slice * d.lanes * V;
+  for (int c = threadIdx.x; c < min(d.lanes * V, d.c - c0); c += blockDim.x) {
+    const Pair t = sums_of<V>(table, c);
+    part[((long)at.n * d.chunks + at.chunk) * d.c + c0 + c] =
+        make_float2(t.a, t.b);
+  }
+}
+
+// All of it in one pass over a slab of whole samples: x and dy stay in
+// registers between the sums and dx.
 template <typename T, int V, int I, int P, bool SILU_>
-__global__ void __launch_bounds__(SLAB) bwd_slab_kernel(
+__global__ void __launch_bounds__(SPAN) bwd_slab_kernel(
     const T* __restrict__ dy, const T* __restrict__ x,
     const T* __restrict__ res, const unsigned char* __restrict__ mask,
     const double2* __restrict__ stats, const float* __restrict__ gamma,
     const float* __restrict__ beta, float2* __restrict__ channel,
     T* __restrict__ dx, T* __restrict__ dres, Slab d) {
-  __shared__ Pair table[SLAB * V];
-  __shared__ Pair group[SLAB];
+  __shared__ float table[2 * SPAN * V];
+  __shared__ Pair group[SPAN];
   const Spot at(d, V);
-  const long base = (long)at.n * d.hw * d.c + at.first + at.lane * V;
   Vec<T, V> a[I], g[I];
-  unsigned bits[I];
+  unsigned char bits[I];
 #pragma unroll
   for (int k = 0; k < I; ++k) {
-    const int row = at.r + k * d.rows;
-    if (at.on && row < d.hw) {
-      const long i = base + (long)row * d.c;
-      a[k] = load<T, V>(x + i);
-      g[k] = load<T, V>(dy + i);
-      if (!SILU_ && mask) bits[k] = mask[i / V];
+    if (at.has(k, d)) {
+      a[k] = load<T, V>(at.row(x, k));
+      g[k] = load<T, V>(at.row(dy, k));
+      if (!SILU_ && mask) bits[k] = *at.template bits<V>(mask, k);
     }
   }
-  // mean, rstd, s1 and s2 of a thread's channels: one, or P
-  const double2* sample = stats + (long)at.n * d.groups;
-  const int c0 = at.on ? at.first + at.lane * V : 0;
-  float mean[P], rstd[P], gam[V], bet[SILU_ ? V : 1];
-#pragma unroll
-  for (int j = 0; j < P; ++j) {
-    const double2 st = sample[(c0 + j) / d.cpg];
-    mean[j] = (float)st.x;
-    rstd[j] = (float)st.y;
-  }
-#pragma unroll
-  for (int j = 0; j < V; ++j) {
-    gam[j] = gamma[c0 + j];
-    if (SILU_) bet[j] = beta[c0 + j];
-  }
-  auto slope = [&](int j, float off, float r) {
-    const float z = fmaf(off * rstd[P == 1 ? 0 : j], gam[j], bet[j]) + r;
-    const float s = sigmoid(z);
-    return s * fmaf(z, 1.f - s, 1.f);
-  };
-  // sums of dz and of dz (x - mean); the latter's rstd comes at the end
+  const Channels<T, V, P, SILU_> ch(at, d, stats, gamma, beta);
   float s[2 * V] = {};
 #pragma unroll
   for (int k = 0; k < I; ++k) {
-    const int row = at.r + k * d.rows;
-    if (at.on && row < d.hw) {
-      const long i = base + (long)row * d.c;
+    if (at.has(k, d)) {
       Vec<T, V> b;
-      if (SILU_ && res) b = load<T, V>(res + i);
+      if (SILU_ && res) b = load<T, V>(at.row(res, k));
       if (!SILU_ && mask) keep<T, V>(g[k], bits[k]);
-#pragma unroll
-      for (int j = 0; j < V; ++j) {
-        const float off = (float)a[k].v[j] - mean[P == 1 ? 0 : j];
-        float dz = (float)g[k].v[j];
-        if (SILU_) {
-          dz *= slope(j, off, res ? (float)b.v[j] : 0.f);
-          b.v[j] = (T)dz;
-        }
-        s[j] += dz;
-        s[V + j] = fmaf(dz, off, s[V + j]);
-      }
-      if (dres) store<T, V>(dres + i, SILU_ ? b : g[k]);
+      ch.add(a[k], g[k], b, res, s);
+      if (dres) store<T, V>(at.row(dres, k), SILU_ ? b : g[k]);
+      in_turn<SILU_>();
     }
   }
-#pragma unroll
-  for (int j = 0; j < V; ++j)
-    table[threadIdx.x * V + j] =
-        Pair{s[j], s[V + j] * rstd[P == 1 ? 0 : j]};
-  __syncthreads();
-  // rows of a channel: first in `parts` shares, in place, then those
+  ch.join(s, table, d);
   const int width = d.lanes * V;
-  const int parts = max(1, (int)blockDim.x / width);
-  for (int u = threadIdx.x; u < width * parts; u += blockDim.x) {
-    const int c = u % width, p = u / width;
-    Pair t = {0.f, 0.f};
-    for (int row = p; row < d.rows; row += parts) t += table[row * width + c];
-    if (p < d.rows) table[u] = t;
-  }
-  __syncthreads();
   for (int c = threadIdx.x; c < width; c += blockDim.x) {
-    Pair t = table[c];
-    for (int p = 1; p < min(parts, d.rows); ++p) t += table[p * width + c];
-    const int to = at.first + c;
+    const Pair t = sums_of<V>(table, c);
+    const int to = at.slice * width + c;
     channel[(long)at.n * d.c + to] = make_float2(t.a, t.b);
     const float f = gamma[to];
-    table[c] = Pair{f * t.a, f * t.b};
+    table[c % V * blockDim.x + c / V] = f * t.a;
+    table[(V + c % V) * blockDim.x + c / V] = f * t.b;
   }
   __syncthreads();
   const float inv = 1.f / ((float)d.hw * (float)d.cpg);
-  add_groups<Pair>(table, 1, d.cpg, d, [&](int q, const Pair& t) {
-    group[q] = Pair{t.a * inv, t.b * inv};
-  });
+  add_groups<Pair>(
+      1, d, [&](int e, int) { return sums_of<V>(table, e); },
+      [&](int q, const Pair& t) { group[q] = Pair{t.a * inv, t.b * inv}; });
   __syncthreads();
   if (!dx || !at.on) return;
   // dx = (rstd gamma) dz - (rstd^2 s2) (x - mean) - rstd s1
   float by_x[P], less[P];
-#pragma unroll
-  for (int j = 0; j < P; ++j) {
-    const Pair t = group[(at.lane * V + j) / d.cpg];
-    by_x[j] = -rstd[j] * rstd[j] * t.b;
-    less[j] = -rstd[j] * t.a;
-  }
+  each_part<P>(at.lane * V, d, [&](int j, int q) {
+    by_x[j] = -ch.rstd[j] * ch.rstd[j] * group[q].b;
+    less[j] = -ch.rstd[j] * group[q].a;
+  });
 #pragma unroll
   for (int k = 0; k < I; ++k) {
-    const int row = at.r + k * d.rows;
-    if (row >= d.hw) break;
-    const long i = base + (long)row * d.c;
+    if (!at.has(k, d)) break;
+    renew<T, V>(a[k]);
+    renew<T, V>(g[k]);
     Vec<T, V> b;
-    if (SILU_ && res) b = load<T, V>(res + i);
+    if (SILU_ && res) b = load<T, V>(at.row(res, k));
+    float out[V];
 #pragma unroll
     for (int j = 0; j < V; ++j) {
       const int p = P == 1 ? 0 : j;
-      const float off = (float)a[k].v[j] - mean[p];
-      float dz = (float)g[k].v[j];
-      if (SILU_) dz *= slope(j, off, res ? (float)b.v[j] : 0.f);
-      a[k].v[j] = (T)fmaf(dz, gam[j] * rstd[p], fmaf(off, by_x[p], less[p]));
+      const float o = ch.off(j, a[k]);
+      float dz = g[k][j];
+      if (SILU_) dz *= ch.slope(j, o, res ? b[j] : 0.f);
+      out[j] = fmaf(dz, ch.scale[j], fmaf(o, by_x[p], less[p]));
     }
-    store<T, V>(dx + i, a[k]);
+    a[k].put(out);
+    store<T, V>(at.row(dx, k), a[k]);
+    in_turn<SILU_>();
   }
 }
 
@@ -399,7 +428,7 @@ std::vector<torch::Tensor> group_norm_bwd(
         cp, dgamma.data_ptr<float>(), dbeta.data_ptr<float>(), s.n, s.c,
         add ? 1 : 0);
   };
-  const Cut slab = cut(s, v, size, BWD_VECTORS);
+  const Cut slab = cut(s, v, size, SPAN, BWD_VECTORS, true);
   if (slab.threads) {
     with_slab(x.scalar_type(), v, slab.vectors, s.cpg % v == 0, [&](auto tag) {
       using G = decltype(tag);
@@ -420,41 +449,57 @@ std::vector<torch::Tensor> group_norm_bwd(
     params();
     return {dx, dres, dgamma, dbeta};
   }
-  const Deal d = deal(s.hw, s.c, v, s.n);
-  auto part = torch::empty({s.n, d.chunks, s.c, 2}, f32);
+  const Cut chunk = chop(s, v, false);
+  const Slab& cd = chunk.d;
+  const long blocks = s.n * cd.slices * cd.chunks;
+  TORCH_CHECK(blocks < (1L << 24), "group_norm: the input is too large");
+  auto part = torch::empty({s.n, cd.chunks, s.c, 2}, f32);
   auto group = torch::empty({s.n, groups, 2}, f32);
-  const dim3 grid((unsigned)(s.n * d.chunks), 1,
-                  (unsigned)((d.cols + d.lanes - 1) / d.lanes));
-  const long all = s.n * groups;
-  const unsigned joins = (unsigned)std::min<long>(all, 1 << 20);
   auto* pt = reinterpret_cast<float2*>(part.data_ptr());
   auto* gp = reinterpret_cast<float2*>(group.data_ptr());
-  int across = 1;
-  while (across < s.cpg && across < JOIN) across *= 2;
-  with_type(x.scalar_type(), v, [&](auto tag) {
+  const auto type = x.scalar_type();
+  const bool inside = s.cpg % v == 0;
+  with_type(type, v, [&](auto tag) {
     using T = typename decltype(tag)::type;
     constexpr int V = decltype(tag)::v;
-    const T* xp = reinterpret_cast<const T*>(x.data_ptr());
-    const T* yp = reinterpret_cast<const T*>(dy.data_ptr());
-    const T* rp = reinterpret_cast<const T*>(r);
     auto sums = [&](auto kernel) {
-      kernel<<<grid, BLOCK, 0, stream>>>(yp, xp, rp, mk, st, gm, bt, pt,
-                                         s.groups, s.cpg, d);
+      kernel<<<(unsigned)blocks, chunk.threads, 0, stream>>>(
+          reinterpret_cast<const T*>(dy.data_ptr()),
+          reinterpret_cast<const T*>(x.data_ptr()),
+          reinterpret_cast<const T*>(r), mk, st, gm, bt, pt, cd);
     };
+    if (inside && act == SILU) sums(bwd_sums_kernel<T, V, 1, true>);
+    else if (inside) sums(bwd_sums_kernel<T, V, 1, false>);
+    else if (act == SILU) sums(bwd_sums_kernel<T, V, V, true>);
+    else sums(bwd_sums_kernel<T, V, V, false>);
+  });
+  // a block for each group, of about four entries a thread
+  const long all = s.n * groups;
+  const unsigned joins = (unsigned)std::min<long>(all, 1 << 20);
+  int across = 1, join = 64;
+  while (across < s.cpg && across < JOIN) across *= 2;
+  while (join < JOIN && (join < across || 4L * join < (long)s.cpg * cd.chunks))
+    join *= 2;
+  bwd_join_kernel<<<joins, join, 0, stream>>>(pt, gm, cp, gp, all, s.groups,
+                                              s.cpg, across, cd);
+  params();
+  if (!dxp && !drp) return {dx, dres, dgamma, dbeta};
+  const Deal d = deal(s.hw, s.c, v, s.n);
+  const dim3 grid((unsigned)(s.n * d.chunks), 1,
+                  (unsigned)((d.cols + d.lanes - 1) / d.lanes));
+  with_type(type, v, [&](auto tag) {
+    using T = typename decltype(tag)::type;
+    constexpr int V = decltype(tag)::v;
     auto apply = [&](auto kernel) {
       kernel<<<grid, BLOCK, 0, stream>>>(
-          yp, xp, rp, mk, st, gm, bt, gp, reinterpret_cast<T*>(dxp),
-          reinterpret_cast<T*>(drp), s.groups, s.cpg, d);
+          reinterpret_cast<const T*>(dy.data_ptr()),
+          reinterpret_cast<const T*>(x.data_ptr()),
+          reinterpret_cast<const T*>(r), mk, st, gm, bt, gp,
+          reinterpret_cast<T*>(dxp), reinterpret_cast<T*>(drp), s.groups,
+          s.cpg, d);
     };
-    if (act == SILU) sums(bwd_sums_kernel<T, V, true>);
-    else sums(bwd_sums_kernel<T, V, false>);
-    bwd_join_kernel<<<joins, JOIN, 0, stream>>>(
-        pt, gm, cp, gp, all, s.groups, s.cpg, across, d);
-    params();
-    if (dxp || drp) {
-      if (act == SILU) apply(bwd_apply_kernel<T, V, true>);
-      else apply(bwd_apply_kernel<T, V, false>);
-    }
+    if (act == SILU) apply(bwd_apply_kernel<T, V, true>);
+    else apply(bwd_apply_kernel<T, V, false>);
   });
   return {dx, dres, dgamma, dbeta};
 }

@@ -211,6 +211,14 @@ GPU_CASES = [
     (1, 40, 40, 1024, 8, "relu", True, "bf16"),
     (700, 1, 1, 256, 8, "silu", False, "bf16"),    # rows of tokens
     (20, 11, 13, 64, 4, "relu", True, "bf16"),
+    (1, 1365, 1, 24, 1, "relu", False, "bf16"),    # rows just past a split
+    (1, 70, 70, 4104, 8, "relu", True, "bf16"),    # groups of 513 channels
+    (2, 7, 5, 8208, 2, "silu", True, "bf16"),      # of 4,104: slices of one
+    (1, 33, 31, 5000, 1, "none", True, "fp16"),
+    (1, 120, 120, 6, 3, "silu", True, "bf16"),
+    (1, 300, 301, 10, 5, "relu", True, "fp32"),
+    (3, 128, 128, 30, 2, "silu", False, "bf16"),
+    (1, 9000, 1, 8, 8, "relu", False, "fp16"),     # a channel a group, long
 ]
 
 
