@@ -119,6 +119,10 @@ def main() -> int:
     ap.add_argument("--dtype", default="bf16", choices=["bf16", "fp32"],
                     help="GPU compute path (fp32 = torch/MIOpen "
                          "full-precision; used for parity runs)")
+    ap.add_argument("--norm", default="batch", choices=["batch", "group"])
+    ap.add_argument("--optimizer", default="sgd", choices=["sgd", "adamw"])
+    ap.add_argument("--state-bits", type=int, default=32, choices=[8, 32],
+                    help="bits of each of AdamW's moments")
     ap.add_argument("--preflight", action="store_true",
                     help="multi-GPU RCCL smoke: 5 steps of every mode with "
                          "per-rank digests printed (run under torchrun on "
@@ -131,6 +135,11 @@ def main() -> int:
     cfg.data.global_batch = None
     cfg.data.batch_size = args.batch
     cfg.compute_dtype = args.dtype
+    cfg.norm = args.norm
+    cfg.optim.optimizer = args.optimizer
+    cfg.optim.state_bits = args.state_bits
+    if args.optimizer == "adamw":
+        cfg.optim.lr = 1e-3
     O.set_compute_dtype(args.dtype)
 
     rank, world, device = init_distributed("auto", backend=args.backend)
@@ -140,9 +149,10 @@ def main() -> int:
         return preflight(rank, world, device)
     torch.manual_seed(cfg.seed)
 
-    model = build_model(cfg.model).to(device)
+    model = build_model(cfg.model, norm=cfg.norm).to(device)
     model.train()
-    space = FlatParamSpace(model, device)
+    space = FlatParamSpace(model, device,
+                           momentum=cfg.optim.optimizer == "sgd")
     engine = build_engine(space, cfg, rank, world, device)
 
     # synthetic data, resident batches (data=synthetic per BASELINE contract)
@@ -226,8 +236,11 @@ def main() -> int:
                 "per_gpu_batch": args.batch,
                 "seq_len": None,
                 "parallelism": f"eventgrad-ring dp{world}",
-                "optimizer": "sgd lr=1e-2 momentum=0.9",
+                "optimizer": ("sgd lr=1e-2 momentum=0.9"
+                              if args.optimizer == "sgd" else
+                              f"adamw lr=1e-3 {args.state_bits}-bit moments"),
                 "trigger": "adaptive horizon=1.01 warmup=30",
+                **({"norm": args.norm} if args.norm != "batch" else {}),
                 "hip_graph": graph is not None,
                 "final_loss": round(float(loss.item()), 4),
             },
