@@ -3,6 +3,8 @@
 namespace eg {
 namespace gn {
 
+constexpr int STATS_AT_ONCE = 4;
+
 // values of a group in `rows` rows of a slab: the group's, or where a slice
 // is one of several in a group those of slice `sub`
 __device__ __forceinline__ double piece(const Slab& d, int v, int rows,
@@ -35,20 +37,16 @@ __global__ void __launch_bounds__(BLOCK) stats_kernel(
   each_part<P>(alone ? 0 : at.lane * V, d, [&](int j, int q) {
     from[j] = (float)row0[(long)(group + q) * d.cpg];
   });
-  const int steps = (at.count + d.rows - 1) / d.rows;
-#pragma unroll 4
-  for (int k = 0; k < steps; ++k) {
-    if (at.has(k, d)) {
-      const Vec<T, V> a = load<T, V>(at.row(x, k));
+  each_row<STATS_AT_ONCE>(at, d, [&](int k) {
+    const Vec<T, V> a = load<T, V>(at.row(x, k));
 #pragma unroll
-      for (int j = 0; j < V; ++j) {
-        const int p = P == 1 ? 0 : j;
-        const float e = a[j] - from[p];
-        s[p] += e;
-        q2[p] = fmaf(e, e, q2[p]);
-      }
+    for (int j = 0; j < V; ++j) {
+      const int p = P == 1 ? 0 : j;
+      const float e = a[j] - from[p];
+      s[p] += e;
+      q2[p] = fmaf(e, e, q2[p]);
     }
-  }
+  });
 #pragma unroll
   for (int j = 0; j < P; ++j) {
     table[j * blockDim.x + threadIdx.x] = s[j];

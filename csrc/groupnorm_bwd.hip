@@ -3,6 +3,8 @@
 namespace eg {
 namespace gn {
 
+constexpr int SUMS_AT_ONCE = 2;
+
 // ---- backward -------------------------------------------------------------
 
 // dz / dy of a SiLU at z
@@ -247,17 +249,13 @@ __global__ void __launch_bounds__(BLOCK) bwd_sums_kernel(
   const Spot at(d, V);
   const Channels<T, V, P, SILU_> ch(at, d, stats, gamma, beta);
   float s[2 * V] = {};
-  const int steps = (at.count + d.rows - 1) / d.rows;
-#pragma unroll 2
-  for (int k = 0; k < steps; ++k) {
-    if (at.has(k, d)) {
-      const Vec<T, V> a = load<T, V>(at.row(x, k));
-      Vec<T, V> g = load<T, V>(at.row(dy, k)), b;
-      if (SILU_ && res) b = load<T, V>(at.row(res, k));
-      if (!SILU_ && mask) keep<T, V>(g, *at.template bits<V>(mask, k));
-      ch.add(a, g, b, res, s);
-    }
-  }
+  each_row<SUMS_AT_ONCE>(at, d, [&](int k) {
+    const Vec<T, V> a = load<T, V>(at.row(x, k));
+    Vec<T, V> g = load<T, V>(at.row(dy, k)), b;
+    if (SILU_ && res) b = load<T, V>(at.row(res, k));
+    if (!SILU_ && mask) keep<T, V>(g, *at.template bits<V>(mask, k));
+    ch.add(a, g, b, res, s);
+  });
   ch.join(s, table, d);
   const int c0 = at.slice * d.lanes * V;
   for (int c = threadIdx.x; c < min(d.lanes * V, d.c - c0); c += blockDim.x) {

@@ -300,7 +300,7 @@ struct Slab {
   int hw, c, lanes, rows;           // lanes: columns of a slice
   int slices, chunks, per_chunk;    // of a sample; rows of a chunk
   int groups, cpg, in_slice;        // groups of the sample and of a slice
-  Div by_lanes, by_slices, by_chunks, by_subs, by_cpg;
+  Div by_lanes, by_rows, by_slices, by_chunks, by_subs, by_cpg;
   // adding a group up: threads for each, entries of a row, and how a thread
   // goes from one of its entries to the next
   int per, shift, w, down, right;
@@ -360,6 +360,21 @@ struct Spot {
     return p + (base + k * step) / V + (size_t)(off / V);
   }
 };
+
+// Calls f(k) for a thread's rows of a chunk: all but the last without asking
+// for each whether it is there, so that the loads of U go out together.
+template <int U, typename F>
+__device__ __forceinline__ void each_row(const Spot& at, const Slab& d, F f) {
+  if (!at.on) return;
+  const int whole = d.by_rows.of(at.count);
+  int k = 0;
+  for (; k + U <= whole; k += U) {
+#pragma unroll
+    for (int u = 0; u < U; ++u) f(k + u);
+  }
+  for (; k < whole; ++k) f(k);
+  if (at.r + whole * d.rows < at.count) f(whole);
+}
 
 // Calls f(j, q) for a vector's parts with the place q of each in its slice's
 // groups: one part, or a channel each.
@@ -664,6 +679,7 @@ static void man(Cut& out, long rows, int top, int w) {
   d.right = d.per % w;
   d.by_w = div_by(w);
   d.by_lanes = div_by(d.lanes);
+  d.by_rows = div_by(d.rows);
   d.by_slices = div_by(d.slices);
   d.by_chunks = div_by(d.chunks);
   d.by_subs = div_by(d.subs);
