@@ -3,7 +3,9 @@
 namespace eg {
 namespace gn {
 
-constexpr int STATS_AT_ONCE = 4;
+// rows that a thread has in flight: on 4x128x128x320 the statistics took 12.1 us
+// with 4 and 12.6 with 8, applying them 14.3 with 4 and 14.8 with 2
+constexpr int STATS_AT_ONCE = 4, APPLY_AT_ONCE = 4;
 
 // values of a group in `rows` rows of a slab: the group's, or where a slice
 // is one of several in a group those of slice `sub`
@@ -104,43 +106,43 @@ __global__ void __launch_bounds__(BLOCK) join_kernel(
   }
 }
 
-template <typename T, int V, int ACT>
+template <typename T, int V, int P, int ACT>
 __global__ void __launch_bounds__(BLOCK) apply_kernel(
     const T* __restrict__ x, const T* __restrict__ res, T* __restrict__ y,
     unsigned char* __restrict__ mask, const double2* __restrict__ stats,
-    const float* __restrict__ gamma, const float* __restrict__ beta,
-    int groups, int cpg, Deal d) {
-  const Place at(d);
-  if (!at.on) return;
-  const int c0 = at.col * V;
-  const double2* sample = stats + (long)at.n * groups;
-  float mean[V], scale[V], shift[V], limit = 0.f;
+    const float* __restrict__ gamma, const float* __restrict__ beta, Slab d) {
+  const Spot at(d, V);
+  const int c0 = at.first;
+  const double2* sample = stats + (long)at.n * d.groups;
+  float mean[P], scale[V], shift[V], limit = 0.f;
+  double rstd[P];
+  each_part<P>(c0, d, [&](int j, int q) {
+    const double2 st = sample[q];
+    mean[j] = (float)st.x;
+    rstd[j] = st.y;
+  });
 #pragma unroll
   for (int j = 0; j < V; ++j) {
-    const double2 st = sample[(c0 + j) / cpg];
-    mean[j] = (float)st.x;
-    scale[j] = (float)(gamma[c0 + j] * st.y);
+    const int p = P == 1 ? 0 : j;
+    scale[j] = (float)(gamma[c0 + j] * rstd[p]);
     shift[j] = beta[c0 + j];
-    limit = fmaxf(limit, fabsf(scale[j] * mean[j]) + 2.f * fabsf(shift[j]));
+    limit = fmaxf(limit, fabsf(scale[j] * mean[p]) + 2.f * fabsf(shift[j]));
   }
   limit *= 0x1p-20f;
-  const long base = ((long)at.n * d.hw + at.begin) * d.c + c0;
-#pragma unroll 2
-  for (int k = at.r; k < at.count; k += d.rows) {
-    const long i = base + (long)k * d.c;
-    Vec<T, V> a = load<T, V>(x + i), b;
-    if (res) b = load<T, V>(res + i);
+  each_row<APPLY_AT_ONCE>(at, d, [&](int k) {
+    Vec<T, V> a = load<T, V>(at.row(x, k)), b;
+    if (res) b = load<T, V>(at.row(res, k));
     auto exact = [&](int j) {
-      const double2 st = sample[(c0 + j) / cpg];
-      const double z = ((double)(float)x[i + j] - st.x) * st.y *
+      const double2 st = sample[d.by_cpg.of(c0 + j)];
+      const double z = ((double)(float)at.row(x, k)[j] - st.x) * st.y *
                            (double)gamma[c0 + j] + (double)beta[c0 + j];
-      return res ? z + (double)(float)res[i + j] : z;
+      return res ? z + (double)(float)at.row(res, k)[j] : z;
     };
-    const unsigned bits = activate<T, V, V, ACT>(a, b, res, mean, scale,
-                                                 shift, limit, exact);
-    store<T, V>(y + i, a);
-    if (ACT == RELU_BITS) mask[i / V] = (unsigned char)bits;
-  }
+    const unsigned bits = activate<T, V, P, ACT>(a, b, res, mean, scale, shift,
+                                                 limit, exact);
+    store<T, V>(at.row(y, k), a);
+    if (ACT == RELU_BITS) *at.template bits<V>(mask, k) = (unsigned char)bits;
+  });
 }
 
 // All of it in one pass over a slab of whole samples.
@@ -262,13 +264,14 @@ static torch::Tensor forward(const torch::Tensor& x,
   const int subs = cd.span * vs == s.cpg ? cd.subs : 1;
   auto part = torch::empty({s.n * s.groups * subs * cd.chunks, 2},
                            x.options().dtype(torch::kFloat32));
-  const Deal d = deal(s.hw, s.c, v, s.n);
-  const dim3 grid((unsigned)(s.n * d.chunks), 1,
-                  (unsigned)((d.cols + d.lanes - 1) / d.lanes));
+  int va = v;
+  const Cut rows = chop(s, va, false);
   const long all = s.n * s.groups;
   const unsigned joins = (unsigned)std::min<long>(all, 1 << 20);
   const long blocks = s.n * cd.slices * cd.chunks;
-  TORCH_CHECK(blocks < (1L << 24), "group_norm: the input is too large");
+  const long applies = s.n * rows.d.slices * rows.d.chunks;
+  TORCH_CHECK(std::max(blocks, applies) < (1L << 24),
+              "group_norm: the input is too large");
   auto* st = reinterpret_cast<double2*>(own.data_ptr());
   auto* pt = reinterpret_cast<float2*>(part.data_ptr());
   const auto type = x.scalar_type();
@@ -288,11 +291,15 @@ static torch::Tensor forward(const torch::Tensor& x,
   with_type(type, v, [&](auto tag) {
     using T = typename decltype(tag)::type;
     constexpr int V = decltype(tag)::v;
-    with_act(act, mk, [&](auto a) {
-      apply_kernel<T, V, decltype(a)::v><<<grid, BLOCK, 0, stream>>>(
+    auto run = [&](auto kernel) {
+      kernel<<<(unsigned)applies, rows.threads, 0, stream>>>(
           reinterpret_cast<const T*>(x.data_ptr()),
           reinterpret_cast<const T*>(r), reinterpret_cast<T*>(y.data_ptr()),
-          mk, st, gm, bt, s.groups, s.cpg, d);
+          mk, st, gm, bt, rows.d);
+    };
+    with_act(act, mk, [&](auto a) {
+      if (s.cpg % v == 0) run(apply_kernel<T, V, 1, decltype(a)::v>);
+      else run(apply_kernel<T, V, V, decltype(a)::v>);
     });
   });
   return y;

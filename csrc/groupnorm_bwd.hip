@@ -3,7 +3,7 @@
 namespace eg {
 namespace gn {
 
-constexpr int SUMS_AT_ONCE = 2;
+constexpr int SUMS_AT_ONCE = 2, APPLY_AT_ONCE = 4;
 
 // ---- backward -------------------------------------------------------------
 
@@ -12,33 +12,6 @@ __device__ __forceinline__ float silu_slope(float z) {
   const float s = sigmoid(z);
   return s * fmaf(z, 1.f - s, 1.f);
 }
-
-// What a thread keeps of its V channels where sums are applied. SILU: dz is dy
-// times the slope at z; without, it is dy where the forward pass left a bit,
-// or everywhere.
-template <typename T, int V, bool SILU_>
-struct Applied {
-  float mean[V], rstd[V], scale[V], shift[SILU_ ? V : 1];
-
-  __device__ __forceinline__ Applied(const double2* sample, int c0,
-                                     const float* gamma, const float* beta,
-                                     int cpg) {
-#pragma unroll
-    for (int j = 0; j < V; ++j) {
-      const double2 st = sample[(c0 + j) / cpg];
-      mean[j] = (float)st.x;
-      rstd[j] = (float)st.y;
-      scale[j] = gamma[c0 + j] * rstd[j];
-      if (SILU_) shift[j] = beta[c0 + j];
-    }
-  }
-
-  __device__ __forceinline__ float dz(int j, float off, float r,
-                                      float dy) const {
-    if (!SILU_) return dy;
-    return dy * silu_slope(fmaf(off, scale[j], shift[j]) + r);
-  }
-};
 
 // A block a group: each channel's sums over the chunks, for dgamma and dbeta,
 // and the group's s1 and s2.
@@ -120,47 +93,6 @@ __global__ void __launch_bounds__(PC* PN) bwd_params_kernel(
   }
 }
 
-template <typename T, int V, bool SILU_>
-__global__ void __launch_bounds__(BLOCK) bwd_apply_kernel(
-    const T* __restrict__ dy, const T* __restrict__ x,
-    const T* __restrict__ res, const unsigned char* __restrict__ mask,
-    const double2* __restrict__ stats, const float* __restrict__ gamma,
-    const float* __restrict__ beta, const float2* __restrict__ group,
-    T* __restrict__ dx, T* __restrict__ dres, int groups, int cpg, Deal d) {
-  const Place at(d);
-  if (!at.on) return;
-  const Applied<T, V, SILU_> ch(stats + (long)at.n * groups, at.col * V,
-                                 gamma, beta, cpg);
-  // dx = (rstd gamma) dz - (rstd^2 s2) (x - mean) - rstd s1
-  float by_x[V], less[V];
-#pragma unroll
-  for (int j = 0; j < V; ++j) {
-    const float2 s = group[(long)at.n * groups + (at.col * V + j) / cpg];
-    by_x[j] = -ch.rstd[j] * ch.rstd[j] * s.y;
-    less[j] = -ch.rstd[j] * s.x;
-  }
-  const long base = ((long)at.n * d.hw + at.begin) * d.c + at.col * V;
-#pragma unroll 2
-  for (int k = at.r; k < at.count; k += d.rows) {
-    const long i = base + (long)k * d.c;
-    const Vec<T, V> a = load<T, V>(x + i);
-    Vec<T, V> g = load<T, V>(dy + i), b, u;
-    if (SILU_ && res) b = load<T, V>(res + i);
-    if (!SILU_ && mask) keep<T, V>(g, mask[i / V]);
-    float dz[V], out[V];
-#pragma unroll
-    for (int j = 0; j < V; ++j) {
-      const float off = a[j] - ch.mean[j];
-      dz[j] = ch.dz(j, off, SILU_ && res ? b[j] : 0.f, g[j]);
-      out[j] = fmaf(dz[j], ch.scale[j], fmaf(off, by_x[j], less[j]));
-    }
-    u.put(out);
-    if (SILU_) g.put(dz);
-    if (dx) store<T, V>(dx + i, u);
-    if (dres) store<T, V>(dres + i, g);
-  }
-}
-
 // What a thread keeps of its channels, and dz from it. SILU: dz is dy times the
 // slope at z; without, it is dy where the forward pass left a bit, or
 // everywhere. P: parts of a vector with a mean of their own.
@@ -238,6 +170,9 @@ __device__ __forceinline__ Pair sums_of(const float* table, int c) {
           table[(V + c % V) * blockDim.x + c / V]};
 }
 
+// dx = (rstd gamma) dz - (rstd^2 s2) (x - mean) - rstd s1 is two fused
+// multiply-adds of what is fixed for a channel.
+
 // Each channel's sums over one chunk of rows.
 template <typename T, int V, int P, bool SILU_>
 __global__ void __launch_bounds__(BLOCK) bwd_sums_kernel(
@@ -263,6 +198,42 @@ __global__ void __launch_bounds__(BLOCK) bwd_sums_kernel(
     part[((long)at.n * d.chunks + at.chunk) * d.c + c0 + c] =
         make_float2(t.a, t.b);
   }
+}
+
+template <typename T, int V, int P, bool SILU_>
+__global__ void __launch_bounds__(BLOCK) bwd_apply_kernel(
+    const T* __restrict__ dy, const T* __restrict__ x,
+    const T* __restrict__ res, const unsigned char* __restrict__ mask,
+    const double2* __restrict__ stats, const float* __restrict__ gamma,
+    const float* __restrict__ beta, const float2* __restrict__ group,
+    T* __restrict__ dx, T* __restrict__ dres, Slab d) {
+  const Spot at(d, V);
+  const Channels<T, V, P, SILU_> ch(at, d, stats, gamma, beta);
+  float by_x[P], less[P];
+  each_part<P>(at.first, d, [&](int j, int q) {
+    const float2 s = group[(long)at.n * d.groups + q];
+    by_x[j] = -ch.rstd[j] * ch.rstd[j] * s.y;
+    less[j] = -ch.rstd[j] * s.x;
+  });
+  each_row<APPLY_AT_ONCE>(at, d, [&](int k) {
+    const Vec<T, V> a = load<T, V>(at.row(x, k));
+    Vec<T, V> g = load<T, V>(at.row(dy, k)), b, u;
+    if (SILU_ && res) b = load<T, V>(at.row(res, k));
+    if (!SILU_ && mask) keep<T, V>(g, *at.template bits<V>(mask, k));
+    float dz[V], out[V];
+#pragma unroll
+    for (int j = 0; j < V; ++j) {
+      const int p = P == 1 ? 0 : j;
+      const float o = ch.off(j, a);
+      dz[j] = g[j];
+      if (SILU_) dz[j] *= ch.slope(j, o, res ? b[j] : 0.f);
+      out[j] = fmaf(dz[j], ch.scale[j], fmaf(o, by_x[p], less[p]));
+    }
+    u.put(out);
+    if (SILU_) g.put(dz);
+    if (dx) store<T, V>(at.row(dx, k), u);
+    if (dres) store<T, V>(at.row(dres, k), g);
+  });
 }
 
 // All of it in one pass over a slab of whole samples: x and dy stay in
@@ -317,7 +288,6 @@ __global__ void __launch_bounds__(SPAN) bwd_slab_kernel(
       [&](int q, const Pair& t) { group[q] = Pair{t.a * inv, t.b * inv}; });
   __syncthreads();
   if (!dx || !at.on) return;
-  // dx = (rstd gamma) dz - (rstd^2 s2) (x - mean) - rstd s1
   float by_x[P], less[P];
   each_part<P>(at.lane * V, d, [&](int j, int q) {
     by_x[j] = -ch.rstd[j] * ch.rstd[j] * group[q].b;
@@ -482,22 +452,20 @@ std::vector<torch::Tensor> group_norm_bwd(
                                               s.cpg, across, cd);
   params();
   if (!dxp && !drp) return {dx, dres, dgamma, dbeta};
-  const Deal d = deal(s.hw, s.c, v, s.n);
-  const dim3 grid((unsigned)(s.n * d.chunks), 1,
-                  (unsigned)((d.cols + d.lanes - 1) / d.lanes));
   with_type(type, v, [&](auto tag) {
     using T = typename decltype(tag)::type;
     constexpr int V = decltype(tag)::v;
     auto apply = [&](auto kernel) {
-      kernel<<<grid, BLOCK, 0, stream>>>(
+      kernel<<<(unsigned)blocks, chunk.threads, 0, stream>>>(
           reinterpret_cast<const T*>(dy.data_ptr()),
           reinterpret_cast<const T*>(x.data_ptr()),
           reinterpret_cast<const T*>(r), mk, st, gm, bt, gp,
-          reinterpret_cast<T*>(dxp), reinterpret_cast<T*>(drp), s.groups,
-          s.cpg, d);
+          reinterpret_cast<T*>(dxp), reinterpret_cast<T*>(drp), cd);
     };
-    if (act == SILU) apply(bwd_apply_kernel<T, V, true>);
-    else apply(bwd_apply_kernel<T, V, false>);
+    if (inside && act == SILU) apply(bwd_apply_kernel<T, V, 1, true>);
+    else if (inside) apply(bwd_apply_kernel<T, V, 1, false>);
+    else if (act == SILU) apply(bwd_apply_kernel<T, V, V, true>);
+    else apply(bwd_apply_kernel<T, V, V, false>);
   });
   return {dx, dres, dgamma, dbeta};
 }

@@ -171,31 +171,6 @@ __device__ __forceinline__ unsigned activate(
   return bits;
 }
 
-// How the [HW, C] rows of a sample are dealt out where sums are applied: a
-// block takes one chunk of
-// rows (blockIdx.x counts samples, then chunks) and one tile of columns
-// (blockIdx.z); a thread keeps one column of V channels and takes every
-// `rows`-th row of the chunk.
-struct Deal {
-  int hw, c, cols, lanes, rows, per_chunk, chunks;
-};
-
-struct Place {
-  int n, chunk, begin, count;   // the chunk's first row and its rows
-  int lane, r, col;             // column within the tile, row offset, column
-  bool on;
-  __device__ __forceinline__ explicit Place(const Deal& d) {
-    n = blockIdx.x / d.chunks;
-    chunk = blockIdx.x % d.chunks;
-    begin = chunk * d.per_chunk;
-    count = min(d.per_chunk, d.hw - begin);
-    lane = threadIdx.x % d.lanes;
-    r = threadIdx.x / d.lanes;
-    col = blockIdx.z * d.lanes + lane;
-    on = r < d.rows && col < d.cols;
-  }
-};
-
 struct Pair {
   float a, b;
   __device__ __forceinline__ Pair& operator+=(const Pair& o) {
@@ -507,23 +482,6 @@ __device__ __forceinline__ void statistics(Vec<T, V> (&a)[I],
 }
 
 // ---- host -----------------------------------------------------------------
-
-static Deal deal(long hw, int c, int v, long n) {
-  Deal d;
-  d.hw = (int)hw;
-  d.c = c;
-  d.cols = c / v;
-  d.lanes = std::min(d.cols, BLOCK);
-  d.rows = BLOCK / d.lanes;
-  const long tiles = (d.cols + d.lanes - 1) / d.lanes;
-  // about 2,048 blocks, eight a CU, and no chunk under eight rows a thread
-  const long wanted = std::max<long>(1, 2048 / std::max<long>(1, n * tiles));
-  const long most = std::max<long>(1, hw / (8L * d.rows));
-  const long chunks = std::min(wanted, most);
-  d.per_chunk = (int)((hw + chunks - 1) / chunks);
-  d.chunks = (int)((hw + d.per_chunk - 1) / d.per_chunk);
-  return d;
-}
 
 struct Shape {
   long n, hw;
