@@ -43,11 +43,16 @@ torch::Tensor once(const torch::Tensor& t) {
 // Gradients of gamma and beta go straight into pre-allocated .grad views
 // (added to what is there), like those of the other layers; a standalone
 // parameter gets its gradient from autograd.
+struct Views {
+  torch::Tensor dgamma, dbeta;
+};
+
 struct GroupNorm : torch::autograd::Function<GroupNorm> {
   static Variable forward(AutogradContext* ctx, const Variable& x,
                           const Variable& gamma, const Variable& beta,
-                          const c10::optional<Variable>& residual, long groups,
-                          double eps, long act) {
+                          const c10::optional<Variable>& residual,
+                          const Views& views, long groups, double eps,
+                          long act) {
     auto out = group_norm_fwd(x, gamma, beta, groups, eps, act, residual);
     // a ReLU's gradient needs the bits that the pass left (out[2]) in the
     // residual's place, and without an activation it needs neither
@@ -57,10 +62,9 @@ struct GroupNorm : torch::autograd::Function<GroupNorm> {
     ctx->saved_data["residual"] = residual.has_value();
     ctx->saved_data["groups"] = (int64_t)groups;
     ctx->saved_data["act"] = (int64_t)act;
-    if (gamma.requires_grad() && beta.requires_grad() &&
-        gamma.grad().defined() && beta.grad().defined()) {
-      ctx->saved_data["dgamma"] = gamma.grad();
-      ctx->saved_data["dbeta"] = beta.grad();
+    if (views.dgamma.defined()) {
+      ctx->saved_data["dgamma"] = views.dgamma;
+      ctx->saved_data["dbeta"] = views.dbeta;
     }
     return out[0];
   }
@@ -75,7 +79,7 @@ struct GroupNorm : torch::autograd::Function<GroupNorm> {
     const bool want_r = ctx->saved_data["residual"].toBool() &&
                         ctx->needs_input_grad(3);
     const auto view = ctx->saved_data.find("dgamma");
-    const bool direct = want_g && want_b && view != ctx->saved_data.end();
+    const bool direct = view != ctx->saved_data.end();
     c10::optional<torch::Tensor> dgamma, dbeta;
     if (direct) {
       dgamma = view->second.toTensor();
@@ -92,7 +96,7 @@ struct GroupNorm : torch::autograd::Function<GroupNorm> {
                          want_x, want_r && act, dgamma, dbeta);
     }
     if (want_r && !act) d[1] = dy;
-    variable_list out(7);
+    variable_list out(8);
     if (want_x) out[0] = d[0];
     if (want_g && !direct) out[1] = d[2];
     if (want_b && !direct) out[2] = d[3];
@@ -131,7 +135,18 @@ torch::Tensor group_norm(torch::Tensor x, torch::Tensor gamma,
     refuse(beta, true);
     refuse(res, false);
   }
-  return GroupNorm::apply(x, gamma, beta, residual, groups, eps, act);
+  Views views;
+  if (gamma.requires_grad() && beta.requires_grad() &&
+      gamma.grad().defined() && beta.grad().defined()) {
+    views = {gamma.grad(), beta.grad()};
+    // With the views autograd has nothing to bring gamma and beta, and is not
+    // told of them where x or the residual carries the graph.
+    if (x.requires_grad() || (res.defined() && res.requires_grad())) {
+      gamma = gamma.detach();
+      beta = beta.detach();
+    }
+  }
+  return GroupNorm::apply(x, gamma, beta, residual, views, groups, eps, act);
 }
 
 }  // namespace eg

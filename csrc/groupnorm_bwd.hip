@@ -354,9 +354,8 @@ std::vector<torch::Tensor> group_norm_bwd(
                   "group_norm: gradient views must be contiguous fp32 "
                   "vectors of ", s.c);
   } else {
-    auto both = torch::empty({2, s.c}, f32);
-    dgamma = both[0];
-    dbeta = both[1];
+    dgamma = torch::empty({s.c}, f32);
+    dbeta = torch::empty({s.c}, f32);
   }
   if (x.numel() == 0) {
     if (!add) {

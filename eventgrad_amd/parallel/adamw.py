@@ -168,16 +168,19 @@ class AdamW:
             [self.weight_decay if (decay_1d or len(s) >= 2) else 0.0
              for s in space.shapes], **f32)
         # the kernel's plan: no chunk crosses a tensor
-        rows, first = [], [0]
-        for i, (start, size) in enumerate(zip(space.starts, space.numels)):
-            rows += [(start + o, min(CHUNK, size - o), i)
-                     for o in range(0, size, CHUNK)]
-            first.append(len(rows))
-        self._chunks = torch.tensor(rows, **i64).reshape(-1, 3)
-        self._first = torch.tensor(first, **i64)
+        numels = torch.tensor(space.numels, dtype=torch.int64)
+        counts = (numels + CHUNK - 1) // CHUNK
+        first = torch.nn.functional.pad(counts.cumsum(0), (1, 0))
+        tensor = torch.repeat_interleave(torch.arange(space.sz), counts)
+        into = (torch.arange(len(tensor)) - first[tensor]) * CHUNK
+        starts = torch.tensor(space.starts, dtype=torch.int64)
+        self._chunks = torch.stack(
+            [starts[tensor] + into,
+             (numels[tensor] - into).clamp_max(CHUNK), tensor], 1).to(dev)
+        self._first = first.to(dev)
         self._step = torch.zeros(1, **i64)
         # scratch of the norms, and behind it a counter that ends at zero
-        self._part = torch.zeros(len(rows) + 1, **f32)
+        self._part = torch.zeros(len(tensor) + 1, **f32)
         # of the next step: lr, 1 / (1 - b1^t), 1 / sqrt(1 - b2^t); b1^t, b2^t
         self._coef = torch.zeros(3, **f32)
         self._powers = torch.zeros(2, dtype=torch.float64, device=dev)
