@@ -25,6 +25,11 @@
 // has E = 255 and stands for NaN throughout. E is at least 18 (m) and 34 (v):
 // every value is then a normal number in bfloat16, which holds it exactly.
 
+// What bounds it is memory. 17.4 M weights: 28 bytes each in 72 us, 6.8 TB/s,
+// with 32 bits; 16 1/16 bytes each in 48 us, 5.8 TB/s, with 8. Four values a
+// thread, so that 16 lanes are a block of 64 and its largest value is found
+// without shared memory.
+
 #include "common.h"
 
 #include <c10/core/DeviceGuard.h>
