@@ -20,6 +20,7 @@
 
 #include "common.h"
 
+#include <ATen/hip/EmptyTensor.h>
 #include <c10/core/DeviceGuard.h>
 
 namespace eg {
@@ -480,6 +481,13 @@ __device__ __forceinline__ void statistics(Vec<T, V> (&a)[I],
 }
 
 // ---- host -----------------------------------------------------------------
+
+// A new tensor straight from the allocator: a small call's five or so take
+// as long as its launches, and the way through the dispatcher is half of it.
+static torch::Tensor fresh(at::IntArrayRef sizes, at::ScalarType type,
+                           const torch::Tensor& like) {
+  return at::detail::empty_cuda(sizes, type, like.device(), c10::nullopt);
+}
 
 struct Shape {
   long n, hw;

@@ -233,9 +233,8 @@ static torch::Tensor forward(const torch::Tensor& x,
   using namespace gn;
   TORCH_CHECK(eps >= 0, "group_norm: eps must not be negative");
   const c10::DeviceGuard guard(x.device());
-  auto y = torch::empty_like(x);
-  const auto f64 = x.options().dtype(torch::kFloat64);
-  if (stats) *stats = torch::empty({s.n, s.groups, 2}, f64);
+  auto y = fresh(x.sizes(), x.scalar_type(), x);
+  if (stats) *stats = fresh({s.n, s.groups, 2}, torch::kFloat64, x);
   if (x.numel() == 0) return y;
   const void* r = res.defined() ? res.data_ptr() : nullptr;
   const int size = (int)x.element_size();
@@ -244,7 +243,7 @@ static torch::Tensor forward(const torch::Tensor& x,
   const float* bt = beta.data_ptr<float>();
   unsigned char* mk = nullptr;
   if (mask && act == RELU) {
-    *mask = torch::empty({x.numel() / v}, x.options().dtype(torch::kUInt8));
+    *mask = fresh({x.numel() / v}, torch::kUInt8, x);
     mk = mask->data_ptr<unsigned char>();
   }
   const hipStream_t stream = cur_stream();
@@ -269,13 +268,13 @@ static torch::Tensor forward(const torch::Tensor& x,
     });
     return y;
   }
-  torch::Tensor own = stats ? *stats : torch::empty({s.n, s.groups, 2}, f64);
+  torch::Tensor own =
+      stats ? *stats : fresh({s.n, s.groups, 2}, torch::kFloat64, x);
   int vs = v;       // of the statistics, which may have to be narrower
   const Cut chunk = chop(s, vs, true);
   const Slab& cd = chunk.d;
   const int subs = cd.span * vs == s.cpg ? cd.subs : 1;
-  auto part = torch::empty({s.n * s.groups * subs * cd.chunks, 2},
-                           f64);
+  auto part = fresh({s.n * s.groups * subs * cd.chunks, 2}, torch::kFloat64, x);
   int va = v;
   const Cut rows = chop(s, va, false);
   const long all = s.n * s.groups;

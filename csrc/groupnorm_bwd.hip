@@ -346,10 +346,9 @@ std::vector<torch::Tensor> group_norm_bwd(
   TORCH_CHECK(add == dbeta_out.has_value(),
               "group_norm: dgamma_out and dbeta_out go together");
   const c10::DeviceGuard guard(x.device());
-  const auto f32 = x.options().dtype(torch::kFloat32);
   torch::Tensor dx, dres, dgamma, dbeta;
-  if (want_dx) dx = torch::empty_like(x);
-  if (want_dres) dres = torch::empty_like(x);
+  if (want_dx) dx = fresh(x.sizes(), x.scalar_type(), x);
+  if (want_dres) dres = fresh(x.sizes(), x.scalar_type(), x);
   if (add) {
     dgamma = *dgamma_out;
     dbeta = *dbeta_out;
@@ -360,8 +359,8 @@ std::vector<torch::Tensor> group_norm_bwd(
                   "group_norm: gradient views must be contiguous fp32 "
                   "vectors of ", s.c);
   } else {
-    dgamma = torch::empty({s.c}, f32);
-    dbeta = torch::empty({s.c}, f32);
+    dgamma = fresh({s.c}, torch::kFloat32, x);
+    dbeta = fresh({s.c}, torch::kFloat32, x);
   }
   if (x.numel() == 0) {
     if (!add) {
@@ -394,7 +393,7 @@ std::vector<torch::Tensor> group_norm_bwd(
   const float* gm = gamma.data_ptr<float>();
   const float* bt = beta.data_ptr<float>();
   const hipStream_t stream = cur_stream();
-  auto channel = torch::empty({s.n, s.c, 2}, f32);
+  auto channel = fresh({s.n, s.c, 2}, torch::kFloat32, x);
   auto* cp = reinterpret_cast<float2*>(channel.data_ptr());
   auto params = [&] {
     bwd_params_kernel<<<ceil_div(s.c, PC), PC * PN, 0, stream>>>(
@@ -428,8 +427,8 @@ std::vector<torch::Tensor> group_norm_bwd(
   const Slab& cd = chunk.d;
   const long blocks = s.n * cd.slices * cd.chunks;
   TORCH_CHECK(blocks < (1L << 24), "group_norm: the input is too large");
-  auto part = torch::empty({s.n, cd.chunks, s.c, 2}, f32);
-  auto group = torch::empty({s.n, groups, 2}, f32);
+  auto part = fresh({s.n, cd.chunks, s.c, 2}, torch::kFloat32, x);
+  auto group = fresh({s.n, groups, 2}, torch::kFloat32, x);
   auto* pt = reinterpret_cast<float2*>(part.data_ptr());
   auto* gp = reinterpret_cast<float2*>(group.data_ptr());
   const auto type = x.scalar_type();
