@@ -40,18 +40,30 @@ torch::Tensor once(const torch::Tensor& t) {
   return (*node)({fake})[0];
 }
 
-// Gradients of gamma and beta go straight into pre-allocated .grad views
-// (added to what is there), like those of the other layers; a standalone
-// parameter gets its gradient from autograd.
-struct Views {
-  torch::Tensor dgamma, dbeta;
+// Leaves with gradients already there (views into the flat space) get theirs
+// added in place, like those of the other layers; a standalone parameter gets
+// its gradient from autograd. The leaves are kept, and not their gradients:
+// what .grad is when the backward pass runs is what counts, for it may have
+// been replaced or cleared since.
+struct Direct {
+  torch::Tensor gamma, beta;
 };
+
+bool ready(const torch::Tensor& t) {
+  return t.requires_grad() && t.is_leaf() && t.grad().defined();
+}
+
+void give(const torch::Tensor& leaf, const torch::Tensor& d) {
+  auto& grad = leaf.mutable_grad();
+  if (grad.defined()) grad.add_(d);
+  else grad = d;
+}
 
 struct GroupNorm : torch::autograd::Function<GroupNorm> {
   static Variable forward(AutogradContext* ctx, const Variable& x,
                           const Variable& gamma, const Variable& beta,
                           const c10::optional<Variable>& residual,
-                          const Views& views, long groups, double eps,
+                          const Direct& direct, long groups, double eps,
                           long act) {
     auto out = group_norm_fwd(x, gamma, beta, groups, eps, act, residual);
     // a ReLU's gradient needs the bits that the pass left (out[2]) in the
@@ -62,9 +74,9 @@ struct GroupNorm : torch::autograd::Function<GroupNorm> {
     ctx->saved_data["residual"] = residual.has_value();
     ctx->saved_data["groups"] = (int64_t)groups;
     ctx->saved_data["act"] = (int64_t)act;
-    if (views.dgamma.defined()) {
-      ctx->saved_data["dgamma"] = views.dgamma;
-      ctx->saved_data["dbeta"] = views.dbeta;
+    if (direct.gamma.defined()) {
+      ctx->saved_data["gamma"] = direct.gamma;
+      ctx->saved_data["beta"] = direct.beta;
     }
     return out[0];
   }
@@ -78,12 +90,17 @@ struct GroupNorm : torch::autograd::Function<GroupNorm> {
     const bool want_b = ctx->needs_input_grad(2);
     const bool want_r = ctx->saved_data["residual"].toBool() &&
                         ctx->needs_input_grad(3);
-    const auto view = ctx->saved_data.find("dgamma");
-    const bool direct = view != ctx->saved_data.end();
+    const auto kept = ctx->saved_data.find("gamma");
+    const bool direct = kept != ctx->saved_data.end();
+    torch::Tensor gamma, beta;
     c10::optional<torch::Tensor> dgamma, dbeta;
     if (direct) {
-      dgamma = view->second.toTensor();
-      dbeta = ctx->saved_data["dbeta"].toTensor();
+      gamma = kept->second.toTensor();
+      beta = ctx->saved_data["beta"].toTensor();
+      if (gamma.grad().defined() && beta.grad().defined()) {
+        dgamma = gamma.grad();
+        dbeta = beta.grad();
+      }
     }
     const bool again = at::GradMode::is_enabled();
     torch::Tensor dy;
@@ -94,6 +111,10 @@ struct GroupNorm : torch::autograd::Function<GroupNorm> {
       d = group_norm_bwd(dy, saved[0], saved[3], saved[1], saved[2], groups,
                          act, if_defined(saved[4]), if_defined(saved[5]),
                          want_x, want_r && act, dgamma, dbeta);
+      if (direct && !dgamma) {
+        give(gamma, d[2]);
+        give(beta, d[3]);
+      }
     }
     if (want_r && !act) d[1] = dy;
     variable_list out(8);
@@ -135,18 +156,17 @@ torch::Tensor group_norm(torch::Tensor x, torch::Tensor gamma,
     refuse(beta, true);
     refuse(res, false);
   }
-  Views views;
-  if (gamma.requires_grad() && beta.requires_grad() &&
-      gamma.grad().defined() && beta.grad().defined()) {
-    views = {gamma.grad(), beta.grad()};
-    // With the views autograd has nothing to bring gamma and beta, and is not
-    // told of them where x or the residual carries the graph.
+  Direct direct;
+  if (ready(gamma) && ready(beta)) {
+    direct = {gamma, beta};
+    // Autograd then has nothing to bring gamma and beta, and is not told of
+    // them where x or the residual carries the graph.
     if (x.requires_grad() || (res.defined() && res.requires_grad())) {
       gamma = gamma.detach();
       beta = beta.detach();
     }
   }
-  return GroupNorm::apply(x, gamma, beta, residual, views, groups, eps, act);
+  return GroupNorm::apply(x, gamma, beta, residual, direct, groups, eps, act);
 }
 
 }  // namespace eg

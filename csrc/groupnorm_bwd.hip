@@ -64,11 +64,12 @@ __global__ void __launch_bounds__(JOIN) bwd_join_kernel(
 
 // dgamma and dbeta: each channel's sums over the samples, added to what is
 // there (a gradient's view in the flat space) or put down. 16 channels, a
-// cache line of pairs, by 64 shares of the samples.
+// cache line of pairs, by 64 shares of the samples. dgamma and dbeta may be
+// one, where gamma and beta are.
 constexpr int PC = 16, PN = 64;
 __global__ void __launch_bounds__(PC* PN) bwd_params_kernel(
-    const float2* __restrict__ channel, float* __restrict__ dgamma,
-    float* __restrict__ dbeta, long n, int c, int add) {
+    const float2* __restrict__ channel, float* dgamma, float* dbeta, long n,
+    int c, int add) {
   __shared__ Pair slot[PC * PN / 64][PC];
   const int lane = threadIdx.x % PC, share = threadIdx.x / PC;
   const int ch = blockIdx.x * PC + lane;

@@ -546,3 +546,64 @@ def test_gpu_model_matches_cpu(name):
     with torch.no_grad():
         a, b = cpu(x), gpu(x.to(DEV)).cpu()
     assert ((a - b).norm() / a.norm()).item() < 5e-2
+
+
+@pytest.mark.gpu
+def test_gpu_one_tensor_as_gamma_and_beta():
+    """Its gradient is the sum of both, also where it is added in place."""
+    x, gamma, _, _, dy = (t if t is None else t.to(DEV) for t in
+                          inputs(3, 5, 5, 32, "bf16"))
+    a, b, one, kept = (gamma.clone().requires_grad_(True) for _ in range(4))
+    t = x.clone().requires_grad_(True)
+    O.group_norm(t, a, b, 4, 1e-5, "silu").backward(dy)
+    O.group_norm(t, one, one, 4, 1e-5, "silu").backward(dy)
+    assert torch.equal(one.grad, a.grad + b.grad)
+    kept.grad = torch.zeros_like(kept)
+    O.group_norm(t, kept, kept, 4, 1e-5, "silu").backward(dy)
+    assert torch.equal(kept.grad, a.grad + b.grad)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("x_grad", [False, True])
+def test_gpu_gradients_changed_between_forward_and_backward(x_grad):
+    """The gradient goes where .grad is when the backward pass runs."""
+    x, gamma, beta, _, dy = (t if t is None else t.to(DEV) for t in
+                             inputs(3, 5, 5, 32, "bf16"))
+
+    def leaves():
+        return [p.clone().requires_grad_(True) for p in (gamma, beta)]
+
+    def run(a, b):
+        return O.group_norm(x.clone().requires_grad_(x_grad), a, b, 4)
+
+    want = leaves()
+    run(*want).backward(dy)
+    for case in ("cleared", "half", "replaced"):
+        a, b = leaves()
+        a.grad, b.grad = torch.ones_like(a), torch.ones_like(b)
+        old = a.grad
+        y = run(a, b)
+        a.grad = None if case != "replaced" else torch.full_like(a, 2.0)
+        b.grad = None if case == "cleared" else torch.full_like(b, 3.0)
+        y.backward(dy)
+        assert torch.equal(old, torch.ones_like(old)), case
+        base = [2.0 if case == "replaced" else 0.0,
+                0.0 if case == "cleared" else 3.0]
+        for p, q, c in zip((a, b), want, base):
+            assert torch.equal(p.grad, c + q.grad), case
+
+
+@pytest.mark.gpu
+def test_gpu_computed_parameters_pass_their_gradients_on():
+    """gamma and beta that are no leaves, and keep a gradient themselves."""
+    x, gamma, beta, _, dy = (t if t is None else t.to(DEV) for t in
+                             inputs(3, 5, 5, 32, "bf16"))
+    roots = [p.clone().requires_grad_(True) for p in (gamma, beta)]
+    a, b = (p * 2.0 for p in roots)
+    a.retain_grad(), b.retain_grad()
+    t = x.clone().requires_grad_(True)
+    O.group_norm(t, a, b, 4, 1e-5, "relu").backward(dy, retain_graph=True)
+    first = [p.grad.clone() for p in roots]
+    O.group_norm(t, a, b, 4, 1e-5, "relu").backward(dy)
+    for p, f in zip(roots, first):
+        assert f.any() and torch.equal(p.grad, f + f)
