@@ -276,6 +276,10 @@ def group_norm(x, gamma, beta, groups, eps=1e-5, activation="none",
     the activation are one pass, and so are their gradients. On the CPU x is
     [N, C, H, W].
 
+    Where gamma and beta have gradients already, theirs are added in place,
+    on the stream of the forward pass, as for the other layers; only others
+    come out of torch.autograd.grad.
+
     In a captured region gamma and beta need pre-allocated gradients
     (FlatParamSpace gives them), and x and the residual must not themselves
     be leaves that want one: autograd's own accumulation into a leaf that an

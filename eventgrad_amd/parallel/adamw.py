@@ -267,6 +267,8 @@ class AdamW:
         """On the CPU; with the seed and the step it resumes to the bit."""
         return {"kind": "adamw", "state_bits": self.state_bits,
                 "steps": self.steps, "seed": self.seed,
+                "betas": list(self.betas), "powers": self._powers.tolist(),
+                "corrections": self._coef[1:].tolist(),
                 **{k: t.detach().cpu().clone()
                    for k, t in self._state().items()}}
 
@@ -285,3 +287,7 @@ class AdamW:
         self.seed = int(d["seed"])
         self._step.fill_(int(d["steps"]))
         self._set_corrections(int(d["steps"]) + 1)
+        if list(d["betas"]) == list(self.betas):
+            # as the kernel's products left them, which ** only comes close to
+            self._powers.copy_(torch.tensor(d["powers"], dtype=torch.float64))
+            self._coef[1:].copy_(torch.tensor(d["corrections"]))

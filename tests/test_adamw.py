@@ -356,6 +356,25 @@ def test_state_resumes_to_the_bit(device, bits):
                for x, y in zip(opt.moments(), resumed.moments()))
 
 
+@pytest.mark.parametrize("device", devices())
+def test_state_carries_the_corrections(device):
+    """b^t is a product on the GPU, and a resumed run goes on with the same
+    one; with other betas it is the new ones' power."""
+    space, _m = space_of(device=device)
+    opt = AdamW(space, **HYPER)
+    set_grads(space, 0)
+    for _ in range(60):
+        opt.step()
+    saved = opt.state_dict()
+    resumed = AdamW(space, **HYPER)
+    resumed.load_state_dict(saved)
+    assert resumed._powers.tolist() == opt._powers.tolist()
+    assert resumed._coef.tolist() == opt._coef.tolist()
+    other = AdamW(space, **{**HYPER, "betas": (0.5, 0.75)})
+    other.load_state_dict(saved)
+    assert other._powers.tolist() == [0.5 ** 61, 0.75 ** 61]
+
+
 def test_state_refusals():
     space, _ = space_of()
     opt = AdamW(space, state_bits=8)
