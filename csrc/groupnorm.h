@@ -254,6 +254,9 @@ constexpr int CHUNK_ROWS = 16;     // of a thread, where samples are longer
 constexpr int WIDE_VECTORS = 4;    // of a thread, where there are more
 constexpr int FWD_VECTORS = 16, BWD_VECTORS = 8;   // of a thread, at most
 
+// threads at most in the forward pass, where each has P sums of 64 bits in LDS
+constexpr int fwd_threads(int parts) { return parts > 4 ? SPAN : SLAB; }
+
 // Divisions by what a launch fixes. An integer division is a chain of some 30
 // instructions, and the few of a slab's plan took as long as its first loads.
 struct Div {
@@ -371,8 +374,8 @@ __device__ __forceinline__ void each_part(int channel, const Slab& d, F f) {
 
 // Adds the rows r of a table, eight into one at a time, in place, until at
 // most `most` are left; their number is returned.
-template <int K>
-__device__ __forceinline__ int fold(float* table, const Slab& d, int most) {
+template <int K, typename F>
+__device__ __forceinline__ int fold(F* table, const Slab& d, int most) {
   int rows = d.rows;
 #pragma unroll 1
   for (int l = 0; rows > most; ++l) {
@@ -383,8 +386,8 @@ __device__ __forceinline__ int fold(float* table, const Slab& d, int most) {
     for (int t = threadIdx.x - at * n; t < n; t += blockDim.x) {
       if (at >= step) break;
       for (int k = at; k < K; k += step) {
-        float* e = table + k * blockDim.x + t;
-        float s = e[0];
+        F* e = table + k * blockDim.x + t;
+        F s = e[0];
 #pragma unroll
         for (int i = 1; i < 8; ++i)
           if (t + i * n < all) s += e[i * n];
@@ -425,8 +428,8 @@ __device__ __forceinline__ void add_groups(int rows, const Slab& d, Get get,
 
 // the e-th entry of a row, where a thread's K = P sums are a vector's parts
 template <int P>
-__device__ __forceinline__ float part(const float* table, const Slab& d, int e,
-                                      int row) {
+__device__ __forceinline__ double part(const double* table, const Slab& d,
+                                       int e, int row) {
   return P == 1 ? table[row * d.lanes + e]
                 : table[e % P * blockDim.x + row * d.lanes + e / P];
 }
@@ -434,20 +437,34 @@ __device__ __forceinline__ float part(const float* table, const Slab& d, int e,
 // The means and the sums of squared distances from them of a slab's groups,
 // from the registers. emit(q, mean, m2) is called in one thread a group, with
 // the means in mean_of. P: parts of a vector that have a mean each, 1 where it
-// lies within a group.
-template <typename T, int V, int I, int P, typename Emit>
+// lies within a group. Sums of a vector's values, or of a channel's in one
+// thread, are taken in fp32 and everything beyond in 64 bits. EXACT: only a
+// 16-bit vector's values are added in fp32, and the distances are taken and
+// squared in 64 bits: a ReLU's bits hang on the mean and rstd as much as on z.
+// (With a thread's sums in fp32 these were 1e-8 off, and one in some 20 passes
+// over the 16.8 M values of 256x32x32x64 had a bit wrong. It costs 0.7 us of
+// 10.7 on 100x32x32x64.)
+template <typename T, int V, int I, int P, bool EXACT, typename Emit>
 __device__ __forceinline__ void statistics(Vec<T, V> (&a)[I],
                                            const Spot& at, const Slab& d,
-                                           float* table, double* mean_of,
+                                           double* table, double* mean_of,
                                            float (&mean)[P], Emit emit) {
   const int most = P == 1 ? SLAB : 8;    // as they are, or eight rows
-  float s[P] = {};
-  auto get = [&](int e, int row) { return (double)part<P>(table, d, e, row); };
+  using Sum = std::conditional_t<P == 1 || EXACT, double, float>;
+  Sum s[P] = {};
+  auto get = [&](int e, int row) { return part<P>(table, d, e, row); };
 #pragma unroll
   for (int k = 0; k < I; ++k) {
     if (at.has(k, d)) {
+      if constexpr (P > 1 || (EXACT && sizeof(T) == 4)) {
 #pragma unroll
-      for (int j = 0; j < V; ++j) s[P == 1 ? 0 : j] += a[k][j];
+        for (int j = 0; j < V; ++j) s[P == 1 ? 0 : j] += a[k][j];
+      } else {
+        float t = a[k][0];
+#pragma unroll
+        for (int j = 1; j < V; ++j) t += a[k][j];
+        s[0] += t;
+      }
     }
   }
 #pragma unroll
@@ -456,19 +473,32 @@ __device__ __forceinline__ void statistics(Vec<T, V> (&a)[I],
   add_groups<double>(fold<P>(table, d, most), d, get,
                      [&](int q, double t) { mean_of[q] = t * d.inv; });
   __syncthreads();
+  double mid[P];
   each_part<P>(at.lane * V, d, [&](int j, int q) {
-    mean[j] = (float)mean_of[q];
-    s[j] = 0.f;
+    mid[j] = mean_of[q];
+    mean[j] = (float)mid[j];
+    s[j] = 0;
   });
 #pragma unroll
   for (int k = 0; k < I; ++k) {
     renew<T, V>(a[k]);
     if (at.has(k, d)) {
+      if constexpr (EXACT) {
 #pragma unroll
-      for (int j = 0; j < V; ++j) {
-        const int p = P == 1 ? 0 : j;
-        const float e = a[k][j] - mean[p];
-        s[p] = fmaf(e, e, s[p]);
+        for (int j = 0; j < V; ++j) {
+          const int p = P == 1 ? 0 : j;
+          const double e = a[k][j] - mid[p];
+          s[p] = fma(e, e, s[p]);
+        }
+      } else {
+        float t = 0.f;
+#pragma unroll
+        for (int j = 0; j < V; ++j) {
+          const float e = a[k][j] - mean[P == 1 ? 0 : j];
+          if (P == 1) t = fmaf(e, e, t);
+          else s[j] = fmaf(e, e, (float)s[j]);
+        }
+        if (P == 1) s[0] += t;
       }
     }
   }

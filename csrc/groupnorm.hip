@@ -28,7 +28,7 @@ __device__ __forceinline__ double piece(const Slab& d, int v, int rows,
 template <typename T, int V, int P>
 __global__ void __launch_bounds__(BLOCK) stats_kernel(
     const T* __restrict__ x, double2* __restrict__ part_of, Slab d) {
-  __shared__ float table[2 * BLOCK * P];
+  __shared__ double table[2 * BLOCK * P];
   __shared__ float from_of[BLOCK];
   const Spot at(d, V);
   // entries of a group: its slices, and the chunks of each
@@ -38,18 +38,30 @@ __global__ void __launch_bounds__(BLOCK) stats_kernel(
   const int sub = alone ? at.slice - unit * d.subs : 0;
   const int group = alone ? unit : at.slice * d.in_slice;
   const T* row0 = x + ((long)at.n * d.hw + at.begin) * d.c;
-  float from[P], s[P] = {}, q2[P] = {};
+  // (sums beyond a vector are in 64 bits, or beyond a thread's rows)
+  using Sum = std::conditional_t<P == 1, double, float>;
+  float from[P];
+  Sum s[P] = {}, q2[P] = {};
   each_part<P>(alone ? 0 : at.lane * V, d, [&](int j, int q) {
     from[j] = (float)row0[(long)(group + q) * d.cpg];
   });
   each_row<STATS_AT_ONCE>(at, d, [&](int k) {
     const Vec<T, V> a = load<T, V>(at.row(x, k));
+    float t = 0.f, t2 = 0.f;
 #pragma unroll
     for (int j = 0; j < V; ++j) {
-      const int p = P == 1 ? 0 : j;
-      const float e = a[j] - from[p];
-      s[p] += e;
-      q2[p] = fmaf(e, e, q2[p]);
+      const float e = a[j] - from[P == 1 ? 0 : j];
+      if (P == 1) {
+        t += e;
+        t2 = fmaf(e, e, t2);
+      } else {
+        s[j] += e;
+        q2[j] = fmaf(e, e, (float)q2[j]);
+      }
+    }
+    if (P == 1) {
+      s[0] += t;
+      q2[0] += t2;
     }
   });
 #pragma unroll
@@ -157,12 +169,13 @@ __global__ void __launch_bounds__(BLOCK) apply_kernel(
 // ahead of the sums (28.5 us), lines of 128 bytes with twice the vectors (26.4)
 // and of 32 bytes (32.2) were no better.
 template <typename T, int V, int I, int P, int ACT>
-__global__ void __launch_bounds__(I <= WIDE_VECTORS ? SLAB : SPAN) slab_kernel(
+__global__ void __launch_bounds__(I <= WIDE_VECTORS ? fwd_threads(P)
+                                                    : SPAN) slab_kernel(
     const T* __restrict__ x, const T* __restrict__ res, T* __restrict__ y,
     unsigned char* __restrict__ mask, double2* __restrict__ stats,
     const float* __restrict__ gamma, const float* __restrict__ beta,
     double eps, Slab d) {
-  __shared__ float table[(I <= WIDE_VECTORS ? SLAB : SPAN) * P];
+  __shared__ double table[(I <= WIDE_VECTORS ? fwd_threads(P) : SPAN) * P];
   __shared__ double mean_of[SPAN];
   __shared__ double rstd_of[SPAN];
   const Spot at(d, V);
@@ -177,7 +190,8 @@ __global__ void __launch_bounds__(I <= WIDE_VECTORS ? SLAB : SPAN) slab_kernel(
     scale[j] = gamma[c0 + j];
     shift[j] = beta[c0 + j];
   }
-  statistics<T, V, I, P>(
+  // (a ReLU gives the same values with its bits and without)
+  statistics<T, V, I, P, ACT == RELU || ACT == RELU_BITS>(
       a, at, d, table, mean_of, mean, [&](int q, double mu, double m2) {
         const double rstd = 1.0 / sqrt(m2 * d.inv + eps);
         rstd_of[q] = rstd;
@@ -247,7 +261,8 @@ static torch::Tensor forward(const torch::Tensor& x,
     mk = mask->data_ptr<unsigned char>();
   }
   const hipStream_t stream = cur_stream();
-  const Cut slab = cut(s, v, size, SLAB, FWD_VECTORS, false);
+  const int top = fwd_threads(s.cpg % v ? v : 1);
+  const Cut slab = cut(s, v, size, top, FWD_VECTORS, false);
   if (slab.threads) {
     TORCH_CHECK(s.n * slab.d.slices * slab.threads < (1L << 32),
                 "group_norm: the input is too large");

@@ -607,3 +607,31 @@ def test_gpu_computed_parameters_pass_their_gradients_on():
     O.group_norm(t, a, b, 4, 1e-5, "relu").backward(dy)
     for p, f in zip(roots, first):
         assert f.any() and torch.equal(p.grad, f + f)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("shape,groups", [
+    ((8, 32, 32, 64), 8), ((8, 32, 32, 64), 32), ((64, 8, 8, 36), 4),
+    ((1, 256, 256, 32), 2), ((1, 256, 256, 36), 6), ((40, 7, 7, 30), 6)])
+def test_gpu_relu_gate_hangs_on_exact_statistics(shape, groups):
+    """x is of sixteenths, so that its sums and those of its squares are exact
+    in fp32; the residual takes back all of z that fp32 holds. What is left is
+    2^-25 of z and less, and its sign is that of 64 bits: with the statistics
+    off by 2^-50 of themselves, wherever more is left than 2^-45."""
+    n, h, w, c = shape
+    g = torch.Generator().manual_seed(3)
+    x = (torch.randint(-60, 61, shape, generator=g) / 16.0)
+    gamma = 1 + 0.5 * torch.rand(c, generator=g)
+    beta = torch.randn(c, generator=g)
+    xd = x.double().reshape(n, h * w, groups, c // groups)
+    var, mean = torch.var_mean(xd, (1, 3), correction=0, keepdim=True)
+    z = ((xd - mean) / torch.sqrt(var + 1e-5)).reshape(shape) * \
+        gamma.double() + beta.double()
+    res = -z.float()
+    left = z + res.double()
+    r = res.to(DEV).requires_grad_(True)
+    O.group_norm(x.to(DEV), gamma.to(DEV), beta.to(DEV), groups, 1e-5, "relu",
+                 r).backward(torch.ones(shape, device=DEV))
+    sure = left.abs() > 2.0 ** -45
+    assert sure.double().mean() > 0.9
+    assert torch.equal((r.grad.cpu() > 0)[sure], (left > 0)[sure])
