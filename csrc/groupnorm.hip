@@ -21,7 +21,7 @@ __device__ __forceinline__ double piece(const Slab& d, int v, int rows,
 
 // Each group's mean and sum of squared distances from it over one chunk of
 // rows; about 1,024 blocks, with 4 to 16 rows a thread, since the block's own
-// sums cost as much as some rows. 1x512x512x128 bf16: 67 MB in 14.3 us, 4.7
+// sums cost as much as some rows. 1x512x512x128 bf16: 67 MB in 14.5 us, 4.6
 // TB/s; a form that held its rows in registers and summed once for 48 of them
 // took 21. Distances are first measured from the group's first value in the
 // chunk, which is among those added, so that a large mean costs no digits.
@@ -163,11 +163,12 @@ __global__ void __launch_bounds__(BLOCK) apply_kernel(
 }
 
 // All of it in one pass over a slab of whole samples: 102 MB of
-// 256x32x32x64 bf16 with residual, ReLU and bits in 26.5 us, 3.9 TB/s. All
-// blocks are on the chip at once: they load (to 7 us), add up (2 us) and write
-// in step, and the caches are written back behind them. Loading the residual
-// ahead of the sums (28.5 us), lines of 128 bytes with twice the vectors (26.4)
-// and of 32 bytes (32.2) were no better.
+// 256x32x32x64 bf16 with residual, ReLU and bits in 27.8 us, 3.7 TB/s (26.5
+// with sums in fp32, which are too rough for the bits). All blocks are on the
+// chip at once: they load, add up and write in step, and the caches are
+// written back behind them. Loading the residual ahead of the sums, lines of
+// 128 bytes with twice the vectors and of 32 bytes were no better (28.5, 26.4
+// and 32.2 us to 26.5).
 template <typename T, int V, int I, int P, int ACT>
 __global__ void __launch_bounds__(I <= WIDE_VECTORS ? fwd_threads(P)
                                                     : SPAN) slab_kernel(
