@@ -438,9 +438,9 @@ __device__ __forceinline__ double part(const double* table, const Slab& d,
 // from the registers. emit(q, mean, m2) is called in one thread a group, with
 // the means in mean_of. P: parts of a vector that have a mean each, 1 where it
 // lies within a group. Sums of a vector's values, or of a channel's in one
-// thread, are taken in fp32 and everything beyond in 64 bits. EXACT: only a
-// 16-bit vector's values are added in fp32, and the distances are taken and
-// squared in 64 bits: a ReLU's bits hang on the mean and rstd as much as on z.
+// thread, are taken in fp32 and everything beyond in 64 bits. EXACT: all sums,
+// the distances and their squares are in 64 bits: a ReLU's bits hang on the
+// mean and rstd as much as on z.
 // (With a thread's sums in fp32 these were 1e-8 off, and one in some 20 passes
 // over the 16.8 M values of 256x32x32x64 had a bit wrong. It costs 0.7 us of
 // 10.7 on 100x32x32x64.)
@@ -456,7 +456,7 @@ __device__ __forceinline__ void statistics(Vec<T, V> (&a)[I],
 #pragma unroll
   for (int k = 0; k < I; ++k) {
     if (at.has(k, d)) {
-      if constexpr (P > 1 || (EXACT && sizeof(T) == 4)) {
+      if constexpr (P > 1 || EXACT) {
 #pragma unroll
         for (int j = 0; j < V; ++j) s[P == 1 ? 0 : j] += a[k][j];
       } else {

@@ -635,3 +635,55 @@ def test_gpu_relu_gate_hangs_on_exact_statistics(shape, groups):
     sure = left.abs() > 2.0 ** -45
     assert sure.double().mean() > 0.9
     assert torch.equal((r.grad.cpu() > 0)[sure], (left > 0)[sure])
+
+
+def cancelled(shape, groups, dtype, seed):
+    """Inputs under which z is what fp32 leaves of it at many places, and z in
+    64 bits with the absolute sum of its terms.
+
+    In fp32 the residual takes back all of z that fp32 holds. In 16 bits,
+    where a residual has too few digits, beta does it for the value that a
+    channel has at one of its places, and with it for every place of the
+    channel with the same value. The values' sums are not exact in fp32."""
+    n, h, w, c = shape
+    g = torch.Generator().manual_seed(seed)
+    rnd = lambda *s: torch.randn(*s, generator=g)  # noqa: E731
+    x = (rnd(n, h, w, c) * torch.exp(0.5 * rnd(c)) + rnd(c)).to(TYPES[dtype])
+    gamma, beta = 1 + 0.5 * torch.rand(c, generator=g), rnd(c)
+    xd = x.double().reshape(n, h * w, groups, c // groups)
+    mean = xd.mean((1, 3), keepdim=True)
+    rstd = 1 / torch.sqrt(((xd - mean) ** 2).mean((1, 3), keepdim=True) + 1e-5)
+    norm = ((xd - mean) * rstd).reshape(shape) * gamma.double()
+    terms = ((xd.abs() + mean.abs()) * rstd).reshape(shape) * gamma.double()
+    if dtype == "fp32":
+        res = -(norm + beta.double()).float()
+    else:
+        at = torch.randint(0, h * w, (c,), generator=g)
+        beta = -norm[0].reshape(h * w, c)[at, torch.arange(c)].float()
+        res = torch.zeros_like(x)
+    z = norm + beta.double() + res.double()
+    return x, gamma, beta, res, z, terms + beta.double().abs() + res.double().abs()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", ["bf16", "fp16", "fp32"])
+@pytest.mark.parametrize("shape,groups", [
+    ((1, 128, 128, 64), 8), ((1, 128, 128, 256), 2),   # long: whole vectors
+    ((1, 128, 128, 320), 32), ((2, 150, 150, 30), 6),  # across them
+    ((1, 40, 50, 8208), 2),                            # slices of one group
+    ((4, 32, 32, 64), 8), ((4, 16, 16, 36), 4)])       # slabs
+def test_gpu_relu_gate_with_sums_that_round(shape, groups, dtype):
+    """z is at most 2^-24 of its terms at many places, and its bit there hangs
+    on the mean and rstd to as many digits. All of their sums are in 64 bits:
+    a chain of under 1,024 additions, each off by 2^-53 of the sum, twice over
+    for the mean and the squares. 2^-40 of the terms is four times that."""
+    x, gamma, beta, res, z, terms = cancelled(shape, groups, dtype, 7)
+    r = res.to(DEV).requires_grad_(True)
+    O.group_norm(x.to(DEV), gamma.to(DEV), beta.to(DEV), groups, 1e-5, "relu",
+                 r).backward(torch.ones(shape, device=DEV, dtype=x.dtype))
+    sure = z.abs() > 2.0 ** -40 * terms
+    next_to = sure & (z.abs() <= 2.0 ** -24 * terms)
+    assert int(next_to.sum()) >= 30 and sure.double().mean() > 0.999
+    wrong = (r.grad.cpu() > 0) != (z > 0)
+    assert not wrong[sure].any(), \
+        f"{int(wrong[sure].sum())} of {int(next_to.sum())}"
