@@ -4,6 +4,7 @@
 #include <torch/csrc/autograd/functions/basic_ops.h>
 #include <torch/extension.h>
 
+#include <c10/core/AutogradState.h>
 #include <c10/hip/HIPGraphsC10Utils.h>
 
 #include <vector>
@@ -136,6 +137,12 @@ torch::Tensor group_norm(torch::Tensor x, torch::Tensor gamma,
                          c10::optional<torch::Tensor> residual, long groups,
                          double eps, long act) {
   const torch::Tensor res = residual ? *residual : torch::Tensor();
+  // a tangent would be dropped wherever the call does not go through the node
+  if (c10::AutogradState::get_tls_state().get_fw_grad_mode())
+    for (const auto* t : std::initializer_list<const torch::Tensor*>{
+             &x, &gamma, &beta, &res})
+      TORCH_CHECK_NOT_IMPLEMENTED(!t->defined() || !t->_fw_grad(0).defined(),
+                                  "group_norm has no forward-mode derivative");
   const bool wanted =
       at::GradMode::is_enabled() &&
       (x.requires_grad() || gamma.requires_grad() || beta.requires_grad() ||

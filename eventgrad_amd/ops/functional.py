@@ -280,6 +280,9 @@ def group_norm(x, gamma, beta, groups, eps=1e-5, activation="none",
     on the stream of the forward pass, as for the other layers; only others
     come out of torch.autograd.grad.
 
+    On the GPU there is no second derivative and no forward-mode one: asking
+    for either raises.
+
     In a captured region gamma and beta need pre-allocated gradients
     (FlatParamSpace gives them), and x and the residual must not themselves
     be leaves that want one: autograd's own accumulation into a leaf that an

@@ -687,3 +687,40 @@ def test_gpu_relu_gate_with_sums_that_round(shape, groups, dtype):
     wrong = (r.grad.cpu() > 0) != (z > 0)
     assert not wrong[sure].any(), \
         f"{int(wrong[sure].sum())} of {int(next_to.sum())}"
+
+
+def _dual_calls(device, call):
+    """Each of the inputs in turn with a tangent, with frozen parameters,
+    trained ones and those that have a gradient already, with and without
+    recorded gradients: none may come out as if it had no derivative."""
+    import torch.autograd.forward_ad as fw
+    x = torch.randn(2, 3, 3, 8, device=device).bfloat16()
+    for trained in (False, True):
+        for at in range(4):
+            v = [x, torch.ones(8, device=device), torch.ones(8, device=device),
+                 x.clone()]
+            for p in v[1:3]:
+                p.requires_grad_(trained)
+                p.grad = torch.zeros_like(p) if trained else None
+            for grad in (True, False):
+                with fw.dual_level(), torch.set_grad_enabled(grad):
+                    args = list(v)
+                    args[at] = fw.make_dual(v[at], torch.ones_like(v[at]))
+                    with pytest.raises(NotImplementedError,
+                                       match="forward-mode"):
+                        call(*args)
+
+
+def test_forward_mode_is_refused():
+    """The check comes before the one for the device."""
+    from eventgrad_amd.ops.backend import native, native_available
+    if not native_available():
+        pytest.skip("the extension is not built")
+    _dual_calls("cpu", lambda x, a, b, r: native().group_norm(
+        x, a, b, r, 2, 1e-5, 1))
+
+
+@pytest.mark.gpu
+def test_gpu_forward_mode_is_refused():
+    _dual_calls(DEV, lambda x, a, b, r: O.group_norm(
+        x, a, b, 2, 1e-5, "relu", r))
