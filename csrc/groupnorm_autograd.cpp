@@ -148,23 +148,25 @@ torch::Tensor group_norm(torch::Tensor x, torch::Tensor gamma,
       (x.requires_grad() || gamma.requires_grad() || beta.requires_grad() ||
        (res.defined() && res.requires_grad()));
   if (!wanted) return group_norm_only(x, gamma, beta, groups, eps, act, residual);
+  const bool in_place = ready(gamma) && ready(beta);
   if (c10::hip::currentStreamCaptureStatusMayInitCtx() !=
       c10::hip::CaptureStatus::None) {
-    auto refuse = [](const torch::Tensor& t, bool param) {
-      TORCH_CHECK(!(t.defined() && t.requires_grad() && t.is_leaf() &&
-                    !(param && t.grad().defined())),
+    auto refuse = [](const torch::Tensor& t) {
+      TORCH_CHECK(!(t.defined() && t.requires_grad() && t.is_leaf()),
                   "group_norm: a captured backward pass cannot accumulate "
                   "into this leaf; give gamma and beta pre-allocated "
-                  "gradients, and make x and the residual in the captured "
-                  "region");
+                  "gradients, both of them, and make x and the residual in "
+                  "the captured region");
     };
-    refuse(x, false);
-    refuse(gamma, true);
-    refuse(beta, true);
-    refuse(res, false);
+    refuse(x);
+    refuse(res);
+    if (!in_place) {
+      refuse(gamma);
+      refuse(beta);
+    }
   }
   Direct direct;
-  if (ready(gamma) && ready(beta)) {
+  if (in_place) {
     direct = {gamma, beta};
     // Autograd then has nothing to bring gamma and beta, and is not told of
     // them where x or the residual carries the graph.

@@ -283,10 +283,11 @@ def group_norm(x, gamma, beta, groups, eps=1e-5, activation="none",
     On the GPU there is no second derivative and no forward-mode one: asking
     for either raises.
 
-    In a captured region gamma and beta need pre-allocated gradients
-    (FlatParamSpace gives them), and x and the residual must not themselves
-    be leaves that want one: autograd's own accumulation into a leaf that an
-    eager graph also holds cannot be captured.
+    In a captured region gamma and beta need pre-allocated gradients, both
+    of them (FlatParamSpace gives them), or must both be frozen or computed,
+    and x and the residual must not themselves be leaves that want one:
+    autograd's own accumulation into a leaf that an eager graph also holds
+    cannot be captured.
     """
     if activation not in _ACTIVATIONS:
         raise ValueError(f"activation must be one of "

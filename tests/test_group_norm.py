@@ -724,3 +724,32 @@ def test_forward_mode_is_refused():
 def test_gpu_forward_mode_is_refused():
     _dual_calls(DEV, lambda x, a, b, r: O.group_norm(
         x, a, b, 2, 1e-5, "relu", r))
+
+
+@pytest.mark.gpu
+def test_gpu_capture_refuses_one_trained_parameter():
+    """Gradients are added in place where gamma and beta both have one. With
+    the other frozen, or computed, autograd would accumulate into the leaf."""
+    x = torch.randn(2, 4, 4, 16, device=DEV).bfloat16()
+    trained = torch.ones(16, device=DEV, requires_grad=True)
+    trained.grad = torch.zeros_like(trained)
+    frozen = torch.zeros(16, device=DEV)
+    # frozen parameters are taken, and so are those that both have gradients
+    other = frozen.clone().requires_grad_(True)
+    other.grad = torch.zeros_like(other)
+    O.group_norm(x, frozen, frozen, 4)             # loads the kernels
+    torch.cuda.synchronize()
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        for pair in ((trained, frozen), (frozen, trained)):
+            with pytest.raises(RuntimeError, match="both of them"):
+                O.group_norm(x, *pair, 4)
+        y = O.group_norm(x, trained, other, 4)
+        z = O.group_norm(x, frozen + 1, frozen, 4)
+    g.replay()
+    torch.cuda.synchronize()
+    assert torch.equal(y, z)
+    assert torch.equal(z, O.group_norm(x, frozen + 1, frozen, 4))
+    # and outside of one each keeps its gradient
+    O.group_norm(x, trained, frozen, 4).float().square().sum().backward()
+    assert trained.grad.any()
