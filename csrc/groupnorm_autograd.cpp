@@ -149,8 +149,9 @@ torch::Tensor group_norm(torch::Tensor x, torch::Tensor gamma,
        (res.defined() && res.requires_grad()));
   if (!wanted) return group_norm_only(x, gamma, beta, groups, eps, act, residual);
   const bool in_place = ready(gamma) && ready(beta);
-  if (c10::hip::currentStreamCaptureStatusMayInitCtx() !=
-      c10::hip::CaptureStatus::None) {
+  const bool captured = c10::hip::currentStreamCaptureStatusMayInitCtx() !=
+                        c10::hip::CaptureStatus::None;
+  if (captured) {
     auto refuse = [](const torch::Tensor& t) {
       TORCH_CHECK(!(t.defined() && t.requires_grad() && t.is_leaf()),
                   "group_norm: a captured backward pass cannot accumulate "
@@ -170,10 +171,16 @@ torch::Tensor group_norm(torch::Tensor x, torch::Tensor gamma,
     direct = {gamma, beta};
     // Autograd then has nothing to bring gamma and beta, and is not told of
     // them where x or the residual carries the graph.
-    if (x.requires_grad() || (res.defined() && res.requires_grad())) {
+    const bool carried =
+        x.requires_grad() || (res.defined() && res.requires_grad());
+    if (carried || captured) {
       gamma = gamma.detach();
       beta = beta.detach();
     }
+    // In a captured region a leaf of the call's own carries it: the engine
+    // ends by waiting for its leaves' streams, and one that an eager graph
+    // holds has that graph's, which is not captured.
+    if (captured && !carried) gamma.set_requires_grad(true);
   }
   return GroupNorm::apply(x, gamma, beta, residual, direct, groups, eps, act);
 }

@@ -753,3 +753,31 @@ def test_gpu_capture_refuses_one_trained_parameter():
     # and outside of one each keeps its gradient
     O.group_norm(x, trained, frozen, 4).float().square().sum().backward()
     assert trained.grad.any()
+
+
+@pytest.mark.gpu
+def test_gpu_captured_beside_a_living_eager_graph():
+    """Parameters alone are trained, x is data, and an eager graph of the same
+    parameters lives while the pass is captured."""
+    x, gamma, beta, _, dy = (t if t is None else t.to(DEV) for t in
+                             inputs(3, 5, 5, 32, "bf16"))
+    leaves = [p.clone().requires_grad_(True) for p in (gamma, beta)]
+    for p in leaves:
+        p.grad = torch.zeros_like(p)
+    living = O.group_norm(x, *leaves, 4, 1e-5, "relu")
+    living.backward(dy, retain_graph=True)
+    want = [p.grad.clone() for p in leaves]
+    torch.cuda.synchronize()
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        for p in leaves:
+            p.grad.zero_()
+        O.group_norm(x, *leaves, 4, 1e-5, "relu").backward(dy)
+    for _ in range(3):
+        for p in leaves:
+            p.grad.fill_(7.0)
+        g.replay()
+        torch.cuda.synchronize()
+        assert all(torch.equal(p.grad, w) for p, w in zip(leaves, want))
+    living.backward(dy)
+    assert all(torch.equal(p.grad, w + w) for p, w in zip(leaves, want))
