@@ -73,8 +73,30 @@ def engine_state_dict(engine) -> dict:
     return d
 
 
+def _norm_of(cfg: dict) -> str:
+    """What a run's norm layers are; files without the field hold batch norm."""
+    norm = cfg.get("norm", "batch")
+    return f"group of {cfg['norm_groups']}" if norm == "group" else norm
+
+
+def _check_model(path: str, state: dict, cfg, model) -> None:
+    """The file's model must be the run's: under every norm the parameters
+    have the same names and shapes."""
+    theirs = _norm_of(state.get("config", {}))
+    ours = _norm_of(dataclasses.asdict(cfg))
+    if theirs != ours:
+        raise ValueError(f"{path} holds a model with norm {theirs!r}, "
+                         f"and this run's has {ours!r}")
+    if model is not None and "buffers" in state:
+        odd = set(state["buffers"]) ^ {n for n, _ in model.named_buffers()}
+        if odd:
+            raise ValueError(f"{path} and the model differ in their buffers: "
+                             f"{', '.join(sorted(odd))}")
+
+
 def load_checkpoint(path: str, space, engine, device, model=None) -> dict:
     state = torch.load(path, map_location="cpu", weights_only=False)
+    _check_model(path, state, engine.cfg, model)
     opt = getattr(engine, "opt", None)
     if (opt is not None) != ("optimizer" in state):
         raise ValueError(
@@ -88,8 +110,7 @@ def load_checkpoint(path: str, space, engine, device, model=None) -> dict:
     if model is not None and "buffers" in state:
         bufs = dict(model.named_buffers())
         for name, saved in state["buffers"].items():
-            if name in bufs:
-                bufs[name].copy_(saved.to(bufs[name].device))
+            bufs[name].copy_(saved.to(bufs[name].device))
         for m in model.modules():
             if hasattr(m, "sync_buffers_after_load"):
                 m.sync_buffers_after_load()

@@ -253,3 +253,49 @@ def test_gpu_trainer_runs():
     assert tr.engine.opt.steps == 8 == m.total_passes
     assert torch.isfinite(tr.space.param).all()
     tr.evaluate()
+
+
+def test_checkpoint_of_another_norm_is_refused(tmp_path):
+    """The parameters have the same names and shapes under every norm, so
+    that nothing but the norm itself tells them apart. A refused file leaves
+    the model as it was."""
+    from eventgrad_amd.train.checkpoint import load_checkpoint, save_checkpoint
+    from eventgrad_amd.train.trainer import Trainer
+
+    def trainer(norm, groups=8, bits=32):
+        return Trainer(serial_cfg(tmp_path, model="resnet20", norm=norm,
+                                  norm_groups=groups, bits=bits))
+
+    def load(tr, path):
+        return load_checkpoint(path, tr.space, tr.engine, tr.device,
+                               model=tr.model)
+
+    kinds = {"batch": trainer("batch"), "group8": trainer("group"),
+             "group4": trainer("group", 4)}
+    for k, tr in kinds.items():
+        tr.space.param.normal_()
+        tr.engine.opt.exp_avg.normal_()
+        save_checkpoint(str(tmp_path / k), tr.cfg, 1, 4, tr.space, tr.engine,
+                        model=tr.model)
+    for k, tr in kinds.items():
+        for other in kinds:
+            before = tr.space.param.clone(), tr.engine.opt.exp_avg.clone()
+            if other == k:
+                assert load(tr, str(tmp_path / k))["pass_num"] == 4
+                continue
+            with pytest.raises(ValueError, match="norm"):
+                load(tr, str(tmp_path / other))
+            assert torch.equal(tr.space.param, before[0])
+            assert torch.equal(tr.engine.opt.exp_avg, before[1])
+    # a file from before there was a choice holds a batch-norm model
+    old = torch.load(tmp_path / "batch", weights_only=False)
+    del old["config"]["norm"], old["config"]["norm_groups"]
+    torch.save(old, tmp_path / "old")
+    load(kinds["batch"], str(tmp_path / "old"))
+    with pytest.raises(ValueError, match="norm"):
+        load(kinds["group8"], str(tmp_path / "old"))
+    # and a model whose buffers are not the file's is another one
+    del old["buffers"]["bn.running_mean"]
+    torch.save(old, tmp_path / "less")
+    with pytest.raises(ValueError, match="bn.running_mean"):
+        load(kinds["batch"], str(tmp_path / "less"))
