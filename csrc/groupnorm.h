@@ -124,7 +124,8 @@ __device__ __forceinline__ float sigmoid(float z) {
 }
 
 // y of one vector, and with RELU_BITS a bit for each z that is not below or
-// at zero. mean, scale and shift make z = (x - mean) scale + shift (+ r).
+// at zero. mean, scale and shift make z = (x - mean) scale + shift (+ r); what
+// a mean of 64 bits was rounded by is in the shift.
 // `exact(j)` is the j-th z in 64 bits; it decides where a z is within the
 // rounding of its terms of zero, `limit` being 2^-20 of those that do not
 // change from value to value.

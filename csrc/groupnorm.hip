@@ -136,17 +136,15 @@ __global__ void __launch_bounds__(BLOCK) apply_kernel(
   const int c0 = at.first;
   const double2* sample = stats + (long)at.n * d.groups;
   float mean[P], scale[V], shift[V], limit = 0.f;
-  double rstd[P];
-  each_part<P>(c0, d, [&](int j, int q) {
-    const double2 st = sample[q];
-    mean[j] = (float)st.x;
-    rstd[j] = st.y;
-  });
+  double2 st[P];
+  each_part<P>(c0, d, [&](int j, int q) { st[j] = sample[q]; });
+#pragma unroll
+  for (int j = 0; j < P; ++j) mean[j] = (float)st[j].x;
 #pragma unroll
   for (int j = 0; j < V; ++j) {
     const int p = P == 1 ? 0 : j;
-    scale[j] = (float)(gamma[c0 + j] * rstd[p]);
-    shift[j] = beta[c0 + j];
+    scale[j] = (float)(gamma[c0 + j] * st[p].y);
+    shift[j] = fmaf(-(float)(st[p].x - mean[p]), scale[j], beta[c0 + j]);
     limit = fmaxf(limit, fabsf(scale[j] * mean[p]) + 2.f * fabsf(shift[j]));
   }
   limit *= 0x1p-20f;
@@ -183,6 +181,7 @@ __global__ void __launch_bounds__(I <= WIDE_VECTORS ? fwd_threads(P)
   __shared__ double table[(I <= WIDE_VECTORS ? fwd_threads(P) : SPAN) * P];
   __shared__ double mean_of[SPAN];
   __shared__ double rstd_of[SPAN];
+  __shared__ float low_of[SPAN];    // rstd times what the mean is rounded by
   const Spot at(d, V);
   Vec<T, V> a[I];
 #pragma unroll
@@ -200,6 +199,7 @@ __global__ void __launch_bounds__(I <= WIDE_VECTORS ? fwd_threads(P)
       a, at, d, table, mean_of, mean, [&](int q, double mu, double m2) {
         const double rstd = 1.0 / sqrt(m2 * d.inv + eps);
         rstd_of[q] = rstd;
+        low_of[q] = (float)((mu - (float)mu) * rstd);
         if (stats)
           stats[(long)at.n * d.groups + at.slice * d.in_slice + q] =
               make_double2(mu, rstd);
@@ -207,11 +207,17 @@ __global__ void __launch_bounds__(I <= WIDE_VECTORS ? fwd_threads(P)
   if (!at.on) return;
   float limit = 0.f;
   if (P == 1) {
-    const double rstd = rstd_of[d.by_cpg.of(at.lane * V)];
+    const int q = d.by_cpg.of(at.lane * V);
+    const double rstd = rstd_of[q];
+    const float low = low_of[q];
 #pragma unroll
-    for (int j = 0; j < V; ++j) scale[j] = (float)(scale[j] * rstd);
+    for (int j = 0; j < V; ++j) {
+      shift[j] = fmaf(-low, scale[j], shift[j]);
+      scale[j] = (float)(scale[j] * rstd);
+    }
   } else {
     each_part<P>(at.lane * V, d, [&](int j, int q) {
+      shift[j] = fmaf(-low_of[q], scale[j], shift[j]);
       scale[j] = (float)(scale[j] * rstd_of[q]);
     });
   }

@@ -13,10 +13,20 @@ __device__ __forceinline__ float silu_slope(float z) {
   return s * fmaf(z, 1.f - s, 1.f);
 }
 
+// The mean in the kernels has 32 bits, and `low` is what those of 64 are beyond
+// it: the same for a whole group, so that the sums are put right once they are
+// added, sum dz xh = sum dz (x - mean) rstd - low rstd sum dz, and dx's
+//   -rstd s1 - rstd xh s2 = -rstd (s1 - low rstd s2) - rstd^2 s2 (x - mean)
+// by what stands in the place of s1.
+__device__ __forceinline__ float low_rstd(const double2& st) {
+  return (float)((st.x - (float)st.x) * st.y);
+}
+
 // A block a group: each channel's sums over the chunks, for dgamma and dbeta,
-// and the group's s1 and s2.
+// and the group's s1, less low rstd s2, and s2.
 __global__ void __launch_bounds__(JOIN) bwd_join_kernel(
-    const float2* __restrict__ part, const float* __restrict__ gamma,
+    const float2* __restrict__ part, const double2* __restrict__ stats,
+    const float* __restrict__ gamma,
     float2* __restrict__ channel, float2* __restrict__ group, long groups,
     int per_sample, int cpg, int across, Slab d) {
   // across: threads side by side over channels, a power of two
@@ -28,6 +38,7 @@ __global__ void __launch_bounds__(JOIN) bwd_join_kernel(
   for (long g = blockIdx.x; g < groups; g += gridDim.x) {
     const long n = g / per_sample;
     const int c0 = (int)(g % per_sample) * cpg;
+    const float low = low_rstd(stats[g]);
     float s1 = 0.f, s2 = 0.f;
     for (int b = 0; b < cpg; b += across) {
       const bool on = b + lane < cpg;
@@ -51,6 +62,7 @@ __global__ void __launch_bounds__(JOIN) bwd_join_kernel(
         __syncthreads();
       }
       if (on && share == 0) {
+        s.y = fmaf(-low, s.x, s.y);
         channel[n * d.c + c0 + b + lane] = s;
         s1 = fmaf(gamma[c0 + b + lane], s.x, s1);
         s2 = fmaf(gamma[c0 + b + lane], s.y, s2);
@@ -58,7 +70,8 @@ __global__ void __launch_bounds__(JOIN) bwd_join_kernel(
     }
     s1 = add_block(s1, sums);
     s2 = add_block(s2, sums);
-    if (threadIdx.x == 0) group[g] = make_float2(s1 * inv, s2 * inv);
+    if (threadIdx.x == 0)
+      group[g] = make_float2(fmaf(-low, s2, s1) * inv, s2 * inv);
   }
 }
 
@@ -106,15 +119,19 @@ struct Channels {
                                       const float* __restrict__ gamma,
                                       const float* __restrict__ beta) {
     const double2* sample = stats + (long)at.n * d.groups;
+    float low[P];
     each_part<P>(at.first, d, [&](int j, int q) {
       const double2 st = sample[q];
       mean[j] = (float)st.x;
       rstd[j] = (float)st.y;
+      low[j] = low_rstd(st);
     });
 #pragma unroll
     for (int j = 0; j < V; ++j) {
-      scale[j] = gamma[at.first + j] * rstd[P == 1 ? 0 : j];
-      if (SILU_) shift[j] = beta[at.first + j];
+      const int p = P == 1 ? 0 : j;
+      const float f = gamma[at.first + j];
+      scale[j] = f * rstd[p];
+      if (SILU_) shift[j] = fmaf(-low[p], f, beta[at.first + j]);
     }
   }
 
@@ -143,7 +160,8 @@ struct Channels {
     if (SILU_) b.put(dz);
   }
 
-  // the block's sums of dz and dz xh of each channel, in the table's first row
+  // the block's sums of dz and dz (x - mean) rstd of each channel, in the
+  // table's first row
   __device__ __forceinline__ void join(const float (&s)[2 * V], float* table,
                                        const Slab& d) const {
 #pragma unroll
@@ -171,8 +189,8 @@ __device__ __forceinline__ Pair sums_of(const float* table, int c) {
           table[(V + c % V) * blockDim.x + c / V]};
 }
 
-// dx = (rstd gamma) dz - (rstd^2 s2) (x - mean) - rstd s1 is two fused
-// multiply-adds of what is fixed for a channel.
+// dx = (rstd gamma) dz - (rstd^2 s2) (x - mean) - rstd s1 (s1 less low rstd
+// s2) is two fused multiply-adds of what is fixed for a channel.
 
 // Each channel's sums over one chunk of rows. Bound by vector instructions as
 // much as by memory: 4x128x128x320 bf16 with a SiLU, 84 MB in 22 us at some 20
@@ -254,6 +272,7 @@ __global__ void __launch_bounds__(SPAN) bwd_slab_kernel(
     T* __restrict__ dx, T* __restrict__ dres, Slab d) {
   __shared__ float table[2 * SPAN * V];
   __shared__ Pair group[SPAN];
+  __shared__ float low_of[SPAN];
   const Spot at(d, V);
   Vec<T, V> a[I], g[I];
   unsigned char bits[I];
@@ -265,6 +284,9 @@ __global__ void __launch_bounds__(SPAN) bwd_slab_kernel(
       if (!SILU_ && mask) bits[k] = *at.template bits<V>(mask, k);
     }
   }
+  for (int q = threadIdx.x; q < d.in_slice; q += blockDim.x)
+    low_of[q] = low_rstd(
+        stats[(long)at.n * d.groups + at.slice * d.in_slice + q]);
   const Channels<T, V, P, SILU_> ch(at, d, stats, gamma, beta);
   float s[2 * V] = {};
 #pragma unroll
@@ -281,7 +303,8 @@ __global__ void __launch_bounds__(SPAN) bwd_slab_kernel(
   ch.join(s, table, d);
   const int width = d.lanes * V;
   for (int c = threadIdx.x; c < width; c += blockDim.x) {
-    const Pair t = sums_of<V>(table, c);
+    Pair t = sums_of<V>(table, c);
+    t.b = fmaf(-low_of[d.by_cpg.of(c)], t.a, t.b);
     const int to = at.slice * width + c;
     channel[(long)at.n * d.c + to] = make_float2(t.a, t.b);
     const float f = gamma[to];
@@ -292,7 +315,9 @@ __global__ void __launch_bounds__(SPAN) bwd_slab_kernel(
   const float inv = 1.f / ((float)d.hw * (float)d.cpg);
   add_groups<Pair>(
       1, d, [&](int e, int) { return sums_of<V>(table, e); },
-      [&](int q, const Pair& t) { group[q] = Pair{t.a * inv, t.b * inv}; });
+      [&](int q, const Pair& t) {
+        group[q] = Pair{fmaf(-low_of[q], t.b, t.a) * inv, t.b * inv};
+      });
   __syncthreads();
   if (!dx || !at.on) return;
   float by_x[P], less[P];
@@ -455,7 +480,7 @@ std::vector<torch::Tensor> group_norm_bwd(
   while (across < s.cpg && across < JOIN) across *= 2;
   while (join < JOIN && (join < across || 4L * join < (long)s.cpg * cd.chunks))
     join *= 2;
-  bwd_join_kernel<<<joins, join, 0, stream>>>(pt, gm, cp, gp, all, s.groups,
+  bwd_join_kernel<<<joins, join, 0, stream>>>(pt, st, gm, cp, gp, all, s.groups,
                                               s.cpg, across, cd);
   params();
   if (!dxp && !drp) return {dx, dres, dgamma, dbeta};

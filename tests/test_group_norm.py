@@ -781,3 +781,34 @@ def test_gpu_captured_beside_a_living_eager_graph():
         assert all(torch.equal(p.grad, w) for p, w in zip(leaves, want))
     living.backward(dy)
     assert all(torch.equal(p.grad, w + w) for p, w in zip(leaves, want))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("shape,groups", [
+    ((2, 32, 32, 64), 8), ((3, 16, 16, 36), 4),         # slabs
+    ((1, 150, 150, 16), 2), ((1, 150, 150, 36), 4)])    # long samples
+def test_gpu_large_mean_costs_no_digits(shape, groups):
+    """A mean of a thousand spreads under a ReLU, whose sums are in 64 bits:
+    fp32 has neither the mean nor what x - mean is off by when it is rounded,
+    3e-5 of a spread. x less a rounded mean is exact (both have one exponent),
+    and what the mean was rounded by is at most 2^-14 of a spread; the rest
+    rounds as for a mean of zero, 128 times at most, terms of these sizes."""
+    n, h, w, c = shape
+    g = torch.Generator().manual_seed(11)
+    x = torch.randn(shape, generator=g) + 1000.0
+    gamma, beta = 1 + torch.rand(c, generator=g), torch.zeros(c)
+    dy = torch.randn(shape, generator=g) + 1.0
+    vals, _ = oracle(x, gamma, beta, None, dy, groups, "relu")
+    split = lambda t: t.double().reshape(n, h * w, groups, c // groups)  # noqa: E731
+    total = lambda t: split(t).mean((1, 3), keepdim=True)  # noqa: E731
+    rstd = 1 / torch.sqrt(total((split(x) - total(x)).reshape(shape) ** 2) + 1e-5)
+    xh = ((split(x) - total(x)) * rstd).abs() + 2.0 ** -14
+    d = split((gamma.double() * vals["dres"]).abs())
+    size = {"y": xh.reshape(shape) * gamma.double(),
+            "dbeta": vals["dres"].abs().sum((0, 1, 2)),
+            "dgamma": (vals["dres"].abs() * xh.reshape(shape)).sum((0, 1, 2)),
+            "dx": (rstd * (d + total(d.reshape(shape)) + xh * total(
+                (d * xh).reshape(shape)))).reshape(shape)}
+    got = run_gpu(x, gamma, beta, None, dy, groups, "relu")
+    for name, t in got.items():
+        close(name, t, vals, size)
