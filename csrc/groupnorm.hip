@@ -93,8 +93,9 @@ __global__ void __launch_bounds__(BLOCK) stats_kernel(
 }
 
 // Joins the pieces of each group, a block for each,
-//   M2 = sum (M2_i + count_i mean_i^2) - M mean^2,
-// which in 64 bits leaves 16 digits less those of (mean / spread)^2.
+//   M2 = sum (M2_i + count_i off_i^2) - M off^2,
+// off being measured from the first piece's mean: from zero it would cost the
+// digits of (mean / spread)^2.
 // Mean and rstd are kept in 64 bits: the sign of z decides a ReLU's gradient,
 // and where z is next to zero it is computed again from them.
 __global__ void __launch_bounds__(BLOCK) join_kernel(
@@ -106,6 +107,7 @@ __global__ void __launch_bounds__(BLOCK) join_kernel(
   const double m = (double)d.hw * d.cpg;
   for (long g = blockIdx.x; g < groups; g += gridDim.x) {
     const double2* p = part + g * subs * d.chunks;
+    const double from = p[0].x;
     double s = 0, q = 0;
     for (int i = threadIdx.x; i < subs * d.chunks; i += blockDim.x) {
       const int chunk = i % d.chunks;
@@ -113,14 +115,16 @@ __global__ void __launch_bounds__(BLOCK) join_kernel(
           piece(d, v, min(d.per_chunk, d.hw - chunk * d.per_chunk),
                 i / d.chunks);
       const double2 e = p[i];
-      s += n * e.x;
-      q += e.y + n * e.x * e.x;
+      const double off = e.x - from;
+      s += n * off;
+      q += e.y + n * off * off;
     }
-    const double mean = add_block(s, slot) / m;
-    const double var = add_block(q, slot) / m - mean * mean;
+    const double off = add_block(s, slot) / m;
+    const double var = add_block(q, slot) / m - off * off;
     if (threadIdx.x == 0) {
       // a variance cannot be below zero, and NaN stays NaN
-      stats[g] = make_double2(mean, 1.0 / sqrt((var < 0 ? 0 : var) + eps));
+      stats[g] = make_double2(from + off,
+                              1.0 / sqrt((var < 0 ? 0 : var) + eps));
     }
   }
 }

@@ -812,3 +812,29 @@ def test_gpu_large_mean_costs_no_digits(shape, groups):
     got = run_gpu(x, gamma, beta, None, dy, groups, "relu")
     for name, t in got.items():
         close(name, t, vals, size)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("shape,groups", [
+    ((2, 32, 32, 64), 8), ((3, 16, 16, 36), 4),         # slabs
+    ((1, 150, 150, 16), 2), ((1, 150, 150, 36), 4)])    # long samples
+def test_gpu_huge_mean_keeps_the_spread(shape, groups):
+    """A mean of 2^20 spreads, x in sixteenths of one. Variances are added up
+    from distances, so that 64 bits keep all the digits of a spread that 24
+    have; as mean squares they would leave 53 - 40. What a mean is rounded by
+    is up to 2^-5 of a spread, added to the sizes of the terms."""
+    n, h, w, c = shape
+    g = torch.Generator().manual_seed(12)
+    x = torch.randn(shape, generator=g) + 2.0 ** 20
+    gamma, beta = 1 + torch.rand(c, generator=g), torch.zeros(c)
+    dy = torch.randn(shape, generator=g) + 1.0
+    vals, _ = oracle(x, gamma, beta, None, dy, groups, "relu")
+    split = lambda t: t.double().reshape(n, h * w, groups, c // groups)  # noqa: E731
+    off = split(x) - split(x).mean((1, 3), keepdim=True)
+    xh = (off / off.square().mean((1, 3), keepdim=True).sqrt()).abs()
+    size = {"y": (xh + 2.0 ** -5).reshape(shape) * gamma.double(),
+            "dgamma": (vals["dres"].abs() *
+                       (xh + 2.0 ** -5).reshape(shape)).sum((0, 1, 2))}
+    got = run_gpu(x, gamma, beta, None, dy, groups, "relu")
+    for name in size:
+        close(name, got[name], vals, size)
