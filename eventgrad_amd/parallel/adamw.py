@@ -125,10 +125,10 @@ class AdamW:
 
     step() takes space.grad as it is, updates space.param and the moments,
     and returns the tensors' squared norms [sz]; it does not refresh the bf16
-    weight shadows (space.refresh_shadows does). The learning rate, the step
-    count and the bias corrections live on the space's device, so a step that
-    was captured into a graph counts on and follows a new `lr` when it is
-    replayed.
+    weight shadows (space.refresh_shadows does). The learning rate, the
+    decays, the step count and the bias corrections live on the space's
+    device, so a step that was captured into a graph counts on and follows a
+    new `lr` or `weight_decay` when it is replayed.
     """
 
     def __init__(self, space: FlatParamSpace, lr: float = 1e-3,
@@ -140,14 +140,11 @@ class AdamW:
             raise ValueError(f"betas must be in [0, 1), got {betas}")
         if not 1e-12 <= eps < math.inf:
             raise ValueError(f"eps must be at least 1e-12, got {eps}")
-        if not 0.0 <= weight_decay < math.inf:
-            raise ValueError(f"weight_decay must not be negative, "
-                             f"got {weight_decay}")
         if state_bits not in (8, 32):
             raise ValueError(f"state_bits must be 8 or 32, got {state_bits}")
         self.space = space
         self.betas, self.eps = (b1, b2), float(eps)
-        self.weight_decay, self.decay_1d = float(weight_decay), bool(decay_1d)
+        self.decay_1d = bool(decay_1d)
         self.state_bits, self.seed = state_bits, int(seed)
         dev, n = space.param.device, space.total
         f32 = dict(dtype=torch.float32, device=dev)
@@ -164,9 +161,10 @@ class AdamW:
             self.codes = torch.zeros(2 * n, **u8)
             # for each block of values m's exponent, then v's
             self.exponents = torch.tensor([18, 34], **u8).repeat(n // QBLOCK)
-        self._decay = torch.tensor(
-            [self.weight_decay if (decay_1d or len(s) >= 2) else 0.0
-             for s in space.shapes], **f32)
+        # which tensors decay, and each one's decay
+        self._decays = torch.tensor([bool(decay_1d or len(s) >= 2)
+                                     for s in space.shapes], device=dev)
+        self._decay = torch.zeros(space.sz, **f32)
         # the kernel's plan: no chunk crosses a tensor
         numels = torch.tensor(space.numels, dtype=torch.int64)
         counts = (numels + CHUNK - 1) // CHUNK
@@ -185,6 +183,7 @@ class AdamW:
         self._coef = torch.zeros(3, **f32)
         self._powers = torch.zeros(2, dtype=torch.float64, device=dev)
         self.lr = lr
+        self.weight_decay = weight_decay
         self._set_corrections(1)
 
     # -- scalars -------------------------------------------------------------
@@ -198,6 +197,18 @@ class AdamW:
             raise ValueError(f"lr must not be negative, got {value}")
         self._lr = float(value)
         self._coef[0] = self._lr
+
+    @property
+    def weight_decay(self) -> float:
+        return self._weight_decay
+
+    @weight_decay.setter
+    def weight_decay(self, value: float) -> None:
+        if not 0.0 <= value < math.inf:
+            raise ValueError(f"weight_decay must not be negative, "
+                             f"got {value}")
+        self._weight_decay = float(value)
+        torch.mul(self._decays, self._weight_decay, out=self._decay)
 
     @property
     def steps(self) -> int:

@@ -184,6 +184,8 @@ class CommEngine:
         if self.opt is not None:
             if self.opt.lr != o.lr:
                 self.opt.lr = o.lr
+            if self.opt.weight_decay != o.weight_decay:
+                self.opt.weight_decay = o.weight_decay
             self._last_norms_sq = self.opt.step()
         else:
             self._last_norms_sq = self.K.sgd_step(self.space, o.lr,

@@ -418,3 +418,26 @@ def test_memory_of_8_bits():
                for t in opt.state_dict().values()
                if isinstance(t, torch.Tensor))
     assert held == space.total * 2 + 2 * space.total // 64
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("bits", [8, 32])
+def test_gpu_captured_step_follows_weight_decay(bits):
+    pair = []
+    for _ in range(2):
+        space, model = space_of(device="cuda")
+        set_grads(space, 0)
+        opt = AdamW(space, state_bits=bits, decay_1d=False, **HYPER)
+        opt.step()
+        pair.append((space, opt, model))
+    (sa, a, _), (sb, b, _) = pair
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        a.step()
+    for wd in (0.1, 0.5, 0.0, 0.5):
+        a.weight_decay = b.weight_decay = wd
+        graph.replay()
+        b.step()
+        torch.cuda.synchronize()
+        assert torch.equal(sa.param, sb.param), wd

@@ -299,3 +299,28 @@ def test_checkpoint_of_another_norm_is_refused(tmp_path):
     torch.save(old, tmp_path / "less")
     with pytest.raises(ValueError, match="bn.running_mean"):
         load(kinds["batch"], str(tmp_path / "less"))
+
+
+@pytest.mark.parametrize("device", [
+    "cpu", pytest.param("cuda", marks=pytest.mark.gpu)])
+@pytest.mark.parametrize("decay_1d", [True, False])
+def test_engine_step_follows_weight_decay(device, decay_1d):
+    """As SGD's step does: with gradients of zero a step is the decay alone,
+    the one that the settings hold when it is taken."""
+    dev = torch.device(device)
+    space = FlatParamSpace(build_model("cnn2").to(dev), dev, momentum=False)
+    cfg = RunConfig(mode="serial", optim=adamw(decay_1d=decay_1d))
+    eng = SerialEngine(space, cfg, 0, 1, dev)
+    for wd in (0.01, 0.5, 0.0):
+        cfg.optim.weight_decay = wd
+        before = space.param.clone()
+        eng.step()
+        assert eng.opt.weight_decay == wd
+        for i, shape in enumerate(space.shapes):
+            d = wd if decay_1d or len(shape) > 1 else 0.0
+            got, was = (space.seg(t, i) for t in (space.param, before))
+            # 1 - lr wd and the product round, or lr wd and the fused sum
+            assert torch.allclose(got, was * (1 - cfg.optim.lr * d),
+                                  rtol=2.0 ** -22, atol=0)
+    with pytest.raises(ValueError):
+        eng.opt.weight_decay = -1.0
