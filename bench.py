@@ -32,7 +32,20 @@ from eventgrad_amd.ops import functional as O
 from eventgrad_amd.parallel import FlatParamSpace, build_engine, init_distributed
 
 
-def preflight(rank: int, world: int, device) -> int:
+def settings(args):
+    """The configuration that the flags ask for, of a timed run's step and of
+    preflight's."""
+    cfg = preset("dcifar10-event")
+    cfg.data.global_batch = None
+    cfg.norm = args.norm
+    cfg.optim.optimizer = args.optimizer
+    cfg.optim.state_bits = args.state_bits
+    if args.optimizer == "adamw":
+        cfg.optim.lr = 1e-3
+    return cfg
+
+
+def preflight(rank: int, world: int, device, args) -> int:
     """5-step RCCL smoke of all four modes with per-rank digests.
 
     makes a scaling-run failure diagnosable in one
@@ -43,15 +56,15 @@ def preflight(rank: int, world: int, device) -> int:
 
     ok = True
     for mode in ("cent", "decent", "event", "spevent"):
-        cfg = preset("dcifar10-event")
+        cfg = settings(args)
         cfg.mode = mode
-        cfg.data.global_batch = None
         cfg.data.batch_size = 32
         cfg.trigger.initial_comm_passes = 2   # passes 3-5 use dynamic masks
         torch.manual_seed(cfg.seed)
-        model = build_model(cfg.model).to(device)
+        model = build_model(cfg.model, norm=cfg.norm).to(device)
         model.train()
-        space = FlatParamSpace(model, device)
+        space = FlatParamSpace(model, device,
+                               momentum=cfg.optim.optimizer == "sgd")
         engine = build_engine(space, cfg, rank, world, device)
         g = torch.Generator(device="cpu").manual_seed(1234 + rank)
         x = torch.randn(32, 3, 32, 32, generator=g).to(device)
@@ -129,24 +142,18 @@ def main() -> int:
                          "any multi-GPU box before a scaling run)")
     args = ap.parse_args()
 
-    cfg = preset("dcifar10-event")
+    cfg = settings(args)
     cfg.mode = args.mode
     cfg.model = args.model
-    cfg.data.global_batch = None
     cfg.data.batch_size = args.batch
     cfg.compute_dtype = args.dtype
-    cfg.norm = args.norm
-    cfg.optim.optimizer = args.optimizer
-    cfg.optim.state_bits = args.state_bits
-    if args.optimizer == "adamw":
-        cfg.optim.lr = 1e-3
     O.set_compute_dtype(args.dtype)
 
     rank, world, device = init_distributed("auto", backend=args.backend)
     if device.type != "cuda":
         raise SystemExit("bench.py requires a GPU")
     if args.preflight:
-        return preflight(rank, world, device)
+        return preflight(rank, world, device, args)
     torch.manual_seed(cfg.seed)
 
     model = build_model(cfg.model, norm=cfg.norm).to(device)

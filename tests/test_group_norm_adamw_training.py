@@ -324,3 +324,34 @@ def test_engine_step_follows_weight_decay(device, decay_1d):
                                   rtol=2.0 ** -22, atol=0)
     with pytest.raises(ValueError):
         eng.opt.weight_decay = -1.0
+
+
+def test_preflight_runs_what_the_flags_ask_for(monkeypatch):
+    """bench.py's smoke run of every mode, up to its first engine."""
+    import types
+    import bench
+    seen = {}
+
+    class Built(Exception):
+        pass
+
+    def model(name, **kw):
+        seen["norm"] = kw.get("norm", "batch")
+        return build_model("cnn2")
+
+    def engine(space, cfg, *rest):
+        seen["optim"], seen["space"] = cfg.optim, space
+        raise Built
+
+    monkeypatch.setattr(bench, "build_model", model)
+    monkeypatch.setattr(bench, "build_engine", engine)
+    for norm, optimizer, bits, lr in (("group", "adamw", 8, 1e-3),
+                                      ("batch", "sgd", 32, 1e-2)):
+        args = types.SimpleNamespace(norm=norm, optimizer=optimizer,
+                                     state_bits=bits)
+        with pytest.raises(Built):
+            bench.preflight(0, 1, torch.device("cpu"), args)
+        assert seen["norm"] == norm
+        assert (seen["optim"].optimizer, seen["optim"].state_bits,
+                seen["optim"].lr) == (optimizer, bits, lr)
+        assert (seen["space"].momentum is None) == (optimizer == "adamw")
