@@ -355,3 +355,33 @@ def test_preflight_runs_what_the_flags_ask_for(monkeypatch):
         assert (seen["optim"].optimizer, seen["optim"].state_bits,
                 seen["optim"].lr) == (optimizer, bits, lr)
         assert (seen["space"].momentum is None) == (optimizer == "adamw")
+
+
+@pytest.mark.parametrize("device", [
+    "cpu", pytest.param("cuda", marks=pytest.mark.gpu)])
+@pytest.mark.parametrize("bits", [8, 32])
+def test_checkpoint_holds_all_of_the_state(tmp_path, device, bits):
+    """What a resumed run starts with is what the saved one ended with, to the
+    bit, and one more step on the same gradients is the same step."""
+    from eventgrad_amd.train.trainer import Trainer
+    first = Trainer(serial_cfg(tmp_path, device, epochs=1, bits=bits))
+    first.train()
+    second = Trainer(serial_cfg(tmp_path, device, epochs=2, bits=bits,
+                                resume=True))
+    assert (second.pass_num, second.start_epoch) == (first.pass_num, 2)
+
+    def same():
+        a, b = first.engine.opt, second.engine.opt
+        assert torch.equal(first.space.param, second.space.param)
+        assert all(torch.equal(x, y) for x, y in zip(a.moments(), b.moments()))
+        assert all(torch.equal(getattr(a, k), getattr(b, k)) for k in
+                   ("_step", "_powers", "_coef", "_decay", "codes",
+                    "exponents"))
+        assert a.seed == b.seed
+
+    same()
+    first.space.grad.normal_()
+    second.space.grad.copy_(first.space.grad)
+    for tr in (first, second):
+        tr.engine.step()
+    same()
